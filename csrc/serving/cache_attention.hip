@@ -1,0 +1,398 @@
+// Attention over a paged cache held in 8 bits (e4m3, one scale for each page
+// and head), for single tokens and for chunks of tokens:
+//
+//   s_j = c q . K_j ks_j,  out = sum_j softmax(s)_j V_j vs_j,  lse = log sum e^s
+//
+// over the positions j that a row sees: up to its own, and not further back
+// than the window. Bound by the bytes of the cached codes for single tokens,
+// by the matrix instructions for long chunks.
+//
+// Both products are formed transposed, so that no operand crosses lanes:
+// S^T = K Q^T leaves query row l % 16 and tokens 16 (l / 16) .. + 15 of 64 in
+// lane l, since the rows of K that a matrix instruction takes are chosen as
+// tokens 16 a + 8 c + 4 h + i (a, i: the lane's row 4 a + i). This is just the
+// order in which O^T = V^T P^T takes its second operand, and a lane's running
+// maximum and its factors belong to its own query row. Keys lie [token][dim]
+// and values [dim][token], so that both are read 16 bytes a lane.
+//
+// Codes become q's type for the scores and fp16 for the values: both hold e4m3
+// exactly. The weights are rounded to fp16 (2^-11; bf16 would show in bf16
+// results): they are p vs over the largest p vs so far, so at most 1, and what
+// falls under fp16's range is under 2^-24 of the result. Sums are fp32.
+//
+// A workgroup's 4 waves take turns at tiles of 64 tokens and join in LDS. Long
+// contexts are split over workgroups in chunks of a fixed number of tokens,
+// whose results a second launch joins in their order.
+#include "device.h"
+#include "geometry.h"
+#include "serving.h"
+
+namespace serving {
+namespace {
+
+constexpr int kWaves = 4;
+
+template <typename T>
+struct Codes;
+template <>
+struct Codes<__bf16> {
+  static __device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false);
+    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false);
+    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true);
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+  }
+};
+template <>
+struct Codes<_Float16> {
+  static __device__ __forceinline__ f16x8 widen(uint32_t lo, uint32_t hi) {
+    const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false);
+    const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
+    const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false);
+    const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
+    return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+  }
+};
+
+// 0xFF in the bytes below the n-th of a dword.
+__device__ __forceinline__ uint32_t bytes_below(int n) {
+  return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1u;
+}
+// 0x80 in the bytes that hold e4m3's NaN.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* to, f32x4 v) {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  t4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = (T)v[i];
+  *reinterpret_cast<t4*>(to) = r;
+}
+
+// DT tiles of 16 dimensions, QT tiles of 16 query rows.
+template <typename T, int DT, int QT>
+__global__ __launch_bounds__(kWaves * 64) void attention_kernel(AttentionArgs a) {
+  using x8 = typename Mat<T>::x8;
+  constexpr int KB = DT / 4;  // blocks of 64 dimensions
+  const CacheArgs& c = a.c;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane & 15, g = lane >> 4;
+  const int h = blockIdx.y, split = blockIdx.z;
+  const int group = a.q_heads / c.heads;
+
+  Place p;
+  if (!place_of_slot(a, group, blockIdx.x, p)) return;
+  if (split >= p.splits) return;
+
+  const int page = c.page, dim = c.dim;
+  const int shift = 31 - __clz(page);
+  const int begin = (p.lo & ~(kTile - 1)) + split * a.chunk;
+  const int end = split == p.splits - 1 || begin + a.chunk > p.hi ? p.hi : begin + a.chunk;
+  const int32_t* table = c.table + (p.b < c.batch ? p.b * c.ldt : 0);
+
+  // the lane's query rows, their positions, and their operands
+  x8 q[QT][KB * 2];
+  int pos[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int i = t * 16 + r < p.rows ? t * 16 + r : p.rows - 1;
+    const int tok = (p.local + i) / group, head = h * group + (p.local + i) % group;
+    pos[t] = p.len - p.count + tok;
+    const T* src = (const T*)a.q + (int64_t)(p.row0 + tok) * a.q_row + head * a.q_head;
+#pragma unroll
+    for (int k = 0; k < KB * 2; ++k) {
+      const int d = (k >> 1) * 64 + g * 16 + (k & 1) * 8;
+      q[t][k] = bits_as<x8>(u32x4{0, 0, 0, 0});
+      if (d < dim) q[t][k] = *reinterpret_cast<const x8*>(src + d);
+    }
+  }
+
+  f32x4 acc[QT][DT] = {};
+  float top[QT], sum[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    top[t] = -kInf;
+    sum[t] = 0.f;
+  }
+  const float unit = a.scale * kLog2e;
+
+  for (int base = begin + wave * kTile; base < end; base += kWaves * kTile) {
+    const int tok0 = base + g * 16;  // the lane's 16 tokens for P and V
+    // pages by groups of 16 tokens; one that is out of range gives NaN
+    const int blk = tok0 >> shift;
+    int pid = blk < c.blocks && tok0 < end ? table[blk] : -1;
+    const bool known = pid >= 0 && pid < c.pages && !p.broken;
+    if (pid < 0 || pid >= c.pages) pid = 0;
+    const int pid_k = __shfl(pid, (r >> 2) << 4);
+    const int64_t ph = (int64_t)pid * c.heads + h, ph_k = (int64_t)pid_k * c.heads + h;
+    const uint8_t* kp = c.k + (ph_k * page + ((base + ((r >> 2) << 4)) & (page - 1)) + (r & 3)) * dim + g * 16;
+    const uint8_t* vp = c.v + (ph * dim + r) * page + (tok0 & (page - 1));
+
+    u32x4 kr[4][KB], vr[DT];
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        kr[m][k] = u32x4{0, 0, 0, 0};
+        if (k * 64 + g * 16 < dim) kr[m][k] = *reinterpret_cast<const u32x4*>(kp + m * 4 * dim + k * 64);
+      }
+    float ks = known ? c.k_scale[ph] * unit : __builtin_nanf("");
+    float vs = known ? c.v_scale[ph] : 1.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      vr[d] = u32x4{0, 0, 0, 0};
+      if (d * 16 < dim) vr[d] = *reinterpret_cast<const u32x4*>(vp + (int64_t)d * 16 * page);
+    }
+    if (tok0 >= end) vs = 1.f;
+    const float vlog = __builtin_amdgcn_logf(vs);
+
+    const bool edge = base + kTile > p.first + 1 || (a.window && base <= p.last - a.window);
+    bool odd = false;
+    if (edge) {
+      // values that no row sees are whatever the page held before
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          vr[d][w] &= bytes_below(p.hi - tok0 - 4 * w) & ~bytes_below(p.lo - tok0 - 4 * w);
+          odd |= nan_bytes(vr[d][w]) != 0;
+        }
+      odd = __any(odd);
+    }
+
+    f16x8 pw[QT][2];
+    f16x8 seen[QT][2];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      f32x4 s[4] = {};
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int k = 0; k < KB; ++k) {
+          s[m] = Mat<T>::mfma(Codes<T>::widen(kr[m][k][0], kr[m][k][1]), q[t][2 * k], s[m]);
+          s[m] = Mat<T>::mfma(Codes<T>::widen(kr[m][k][2], kr[m][k][3]), q[t][2 * k + 1], s[m]);
+        }
+      float best = -kInf;
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[m][i] *= ks;
+          if (edge) {
+            const int j = tok0 + m * 4 + i;
+            const bool in = j <= pos[t] && (!a.window || j > pos[t] - a.window);
+            if (!in) s[m][i] = -kInf;
+            seen[t][m >> 1][(m & 1) * 4 + i] = in ? (_Float16)1.f : (_Float16)0.f;
+          }
+          best = fmaxf(best, s[m][i]);
+        }
+      best += vlog;
+      best = fmaxf(best, __shfl_xor(best, 16));
+      best = fmaxf(best, __shfl_xor(best, 32));
+      const float now = fmaxf(top[t], best);
+      const float ref = now == -kInf ? 0.f : now;
+      if (__any(now != top[t])) {
+        const float f = __builtin_amdgcn_exp2f(top[t] - ref);
+        sum[t] *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[t][d] *= f;
+      }
+      top[t] = now;
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = __builtin_amdgcn_exp2f(s[m][i] - ref);
+          sum[t] += e;
+          pw[t][m >> 1][(m & 1) * 4 + i] = (_Float16)(e * vs);
+        }
+    }
+    if (odd) {
+      // a NaN among the values reaches the rows that see it, and no others
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        f32x4 hits[QT] = {};
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          uint32_t w0 = nan_bytes(vr[d][2 * x]) >> 7, w1 = nan_bytes(vr[d][2 * x + 1]) >> 7;
+          vr[d][2 * x] &= ~(w0 * 0xFFu);
+          vr[d][2 * x + 1] &= ~(w1 * 0xFFu);
+          f16x8 is;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            is[i] = (_Float16)(float)(w0 >> (8 * i) & 1u);
+            is[4 + i] = (_Float16)(float)(w1 >> (8 * i) & 1u);
+          }
+#pragma unroll
+          for (int t = 0; t < QT; ++t) hits[t] = Mat<_Float16>::mfma(is, seen[t][x], hits[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (hits[t][i] > 0.f) acc[t][d][i] = __builtin_nanf("");
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const f16x8 v = Codes<_Float16>::widen(vr[d][2 * x], vr[d][2 * x + 1]);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) acc[t][d] = Mat<_Float16>::mfma(v, pw[t][x], acc[t][d]);
+      }
+  }
+
+  // the waves' parts: against one reference, then summed in the waves' order
+  __shared__ float tops[kWaves][QT][16], sums[kWaves][QT][16];
+  __shared__ f32x4 part[kWaves][DT][64];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    sum[t] += __shfl_xor(sum[t], 16);
+    sum[t] += __shfl_xor(sum[t], 32);
+    if (g == 0) {
+      tops[wave][t][r] = top[t];
+      sums[wave][t][r] = sum[t];
+    }
+  }
+  __syncthreads();
+  const bool whole = p.splits == 1;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    float all = tops[0][t][r];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) all = fmaxf(all, tops[w][t][r]);
+    const float ref = all == -kInf ? 0.f : all;
+    float total = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) total += sums[w][t][r] * __builtin_amdgcn_exp2f(tops[w][t][r] - ref);
+    const float f = __builtin_amdgcn_exp2f(top[t] - ref);
+    if (t) __syncthreads();
+#pragma unroll
+    for (int d = 0; d < DT; ++d) part[wave][d][lane] = acc[t][d] * f;
+    __syncthreads();
+    const int i = t * 16 + r;
+    if (i < p.rows) {
+      const int tok = (p.local + i) / group, head = h * group + (p.local + i) % group;
+      if (whole) {
+        const float inv = total != 0.f ? 1.f / total : 0.f;
+        T* out = (T*)a.out + (int64_t)(p.row0 + tok) * a.o_row + head * a.o_head + g * 4;
+#pragma unroll
+        for (int d = wave; d < DT; d += kWaves) {
+          f32x4 o = part[0][d][lane];
+#pragma unroll
+          for (int w = 1; w < kWaves; ++w) o += part[w][d][lane];
+          if (d * 16 < dim) store4(out + d * 16, o * inv);
+        }
+        if (wave == 0 && g == 0)
+          a.lse[(int64_t)(p.row0 + tok) * a.q_heads + head] = (all + __builtin_amdgcn_logf(total)) * kLn2;
+      } else {
+        float* to = a.work + (((int64_t)blockIdx.x * c.heads + h) * a.splits + split) * a.row_tile * (dim + 2);
+        float* row = to + (int64_t)i * dim + g * 4;
+#pragma unroll
+        for (int d = wave; d < DT; d += kWaves) {
+          f32x4 o = part[0][d][lane];
+#pragma unroll
+          for (int w = 1; w < kWaves; ++w) o += part[w][d][lane];
+          if (d * 16 < dim) *reinterpret_cast<f32x4*>(row + d * 16) = o;
+        }
+        if (wave == 0 && g == 0) {
+          to[(int64_t)a.row_tile * dim + 2 * i] = all;
+          to[(int64_t)a.row_tile * dim + 2 * i + 1] = total;
+        }
+      }
+    }
+  }
+}
+
+// Joins the splits of a row: one wave a row, four dimensions a lane.
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
+  const CacheArgs& c = a.c;
+  const int lane = threadIdx.x & 63;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= (int64_t)c.rows * a.q_heads) return;
+  const int row = (int)(at / a.q_heads), head = (int)(at % a.q_heads);
+  const int group = a.q_heads / c.heads, h = head / group, dim = c.dim;
+  Place p;
+  int64_t slot;
+  int i;
+  if (!place_of_row(a, group, row, head, p, slot, i)) return;
+  if (p.splits == 1) return;  // written whole
+
+  const float* from = a.work + (slot * c.heads + h) * a.splits * a.row_tile * (dim + 2);
+  const int64_t step = (int64_t)a.row_tile * (dim + 2);
+  const float* heads = from + (int64_t)a.row_tile * dim + 2 * i;
+  float all = -kInf;
+  for (int s = 0; s < p.splits; ++s) all = fmaxf(all, heads[s * step]);
+  const float ref = all == -kInf ? 0.f : all;
+  float total = 0.f;
+  f32x4 o = {};
+  const int d = lane * 4;
+  for (int s = 0; s < p.splits; ++s) {
+    const float f = __builtin_amdgcn_exp2f(heads[s * step] - ref);
+    total += heads[s * step + 1] * f;
+    if (d < dim) o += *reinterpret_cast<const f32x4*>(from + s * step + (int64_t)i * dim + d) * f;
+  }
+  const float inv = total != 0.f ? 1.f / total : 0.f;
+  if (d < dim) store4((T*)a.out + (int64_t)row * a.o_row + head * a.o_head + d, o * inv);
+  if (lane == 0) a.lse[at] = (all + __builtin_amdgcn_logf(total)) * kLn2;
+}
+
+template <typename T, int DT, int QT>
+hipError_t launch(const AttentionArgs& a, hipStream_t stream) {
+  const dim3 grid((unsigned)slot_count(a), a.c.heads, a.splits);
+  attention_kernel<T, DT, QT><<<grid, kWaves * 64, 0, stream>>>(a);
+  if (hipError_t e = hipGetLastError()) return e;
+  if (a.splits > 1) {
+    const int64_t rows = (int64_t)a.c.rows * a.q_heads;
+    join_kernel<T><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, stream>>>(a);
+  }
+  return hipGetLastError();
+}
+
+template <typename T, int DT>
+hipError_t by_rows(const AttentionArgs& a, hipStream_t stream) {
+  if constexpr (DT <= 8)
+    if (a.row_tile == 32) return launch<T, DT, 2>(a, stream);
+  return launch<T, DT, 1>(a, stream);
+}
+
+template <typename T>
+hipError_t by_dim(const AttentionArgs& a, hipStream_t stream) {
+  if (a.c.dim <= 64) return by_rows<T, 4>(a, stream);
+  if (a.c.dim <= 128) return by_rows<T, 8>(a, stream);
+  return by_rows<T, 16>(a, stream);
+}
+
+}  // namespace
+
+int64_t plan_attention(AttentionArgs& a, int64_t max_seq_len) {
+  const int group = a.q_heads / a.c.heads;
+  const int64_t per_seq = a.c.starts ? (int64_t)a.c.rows * group / (a.c.batch > 0 ? a.c.batch : 1) : group;
+  a.row_tile = per_seq > 16 && a.c.dim <= 128 ? 32 : 16;  // registers
+  const int64_t slots = slot_count(a);
+  int64_t longest = max_seq_len > 0 ? max_seq_len : 1;
+  if (a.window && longest > a.window + kTile + per_seq) longest = a.window + kTile + per_seq;
+  // enough workgroups to fill the card several times over, of at least one
+  // tile a wave
+  const int64_t target = 4096, unit = kTile * kWaves;
+  const int64_t work = slots * a.c.heads;
+  int64_t splits = target / (work > 0 ? work : 1);
+  const int64_t most = (longest + unit - 1) / unit;
+  splits = splits < 1 ? 1 : splits > most ? most : splits;
+  if (splits > 256) splits = 256;
+  a.chunk = (int)(((longest + splits - 1) / splits + unit - 1) / unit * unit);
+  a.splits = (int)((longest + a.chunk - 1) / a.chunk);
+  return a.splits == 1 ? 0 : work * a.splits * a.row_tile * (a.c.dim + 2);
+}
+
+hipError_t launch_cache_attention(const AttentionArgs& a, hipStream_t stream) {
+  return a.dtype == kBF16 ? by_dim<__bf16>(a, stream) : by_dim<_Float16>(a, stream);
+}
+
+}  // namespace serving

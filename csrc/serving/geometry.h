@@ -1,0 +1,164 @@
+// Which rows, tokens and pages a workgroup has. Plain arithmetic, for the
+// kernels and for host checks of it: no result points outside the arrays that
+// its arguments describe, whatever `starts`, `lens` and `table` hold.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "serving.h"
+
+namespace serving {
+
+constexpr int kTile = 64;  // tokens that a wave takes at once
+
+// ---- attention -------------------------------------------------------------
+
+// Rows of a sequence are (token, head) pairs, `row_tile` of them a workgroup.
+struct Place {
+  int b, row0, count, len;  // sequence (batch: the rows behind the last one), its first row, its rows' tokens, its length
+  int tile, local, rows;    // which tile, its first (token, head) row, rows in it
+  int first, last;          // positions of the first and the last of them
+  int lo, hi, splits;       // tokens seen: [lo, hi); workgroups with any
+  bool broken;              // longer than its row of the table: its results are NaN
+};
+
+// Slots of sequence b start at starts[b] group / row_tile + b: enough for its
+// tiles, whatever the lengths, and a rule that a binary search can invert.
+__host__ __device__ inline int64_t first_slot(const AttentionArgs& a, int group, int b) {
+  return (int64_t)a.c.starts[b] * group / a.row_tile + b;
+}
+
+__host__ __device__ inline int64_t slot_count(const AttentionArgs& a) {
+  const int group = a.q_heads / a.c.heads;
+  if (!a.c.starts) return (int64_t)a.c.batch * ((group + a.row_tile - 1) / a.row_tile);
+  return (int64_t)a.c.rows * group / a.row_tile + a.c.batch + 1;
+}
+
+// The rest of `p` from b, count and tile.
+__host__ __device__ inline void fill_place(const AttentionArgs& a, int group, Place& p) {
+  const int room = a.c.blocks * a.c.page;
+  p.len = p.b < a.c.batch ? a.c.lens[p.b] : 0;
+  p.broken = p.len > room;
+  if (p.broken) p.len = room;
+  if (p.len < 0) p.len = 0;
+  p.local = p.tile * a.row_tile;
+  const int all = p.count * group;
+  p.rows = all - p.local < a.row_tile ? all - p.local : a.row_tile;
+  const int before = p.len - p.count;
+  p.first = before + p.local / group;
+  p.last = before + (p.local + p.rows - 1) / group;
+  p.hi = p.last + 1 > 0 ? p.last + 1 : 0;
+  p.lo = a.window && p.first - a.window + 1 > 0 ? p.first - a.window + 1 : 0;
+  const int start = p.lo & ~(kTile - 1);
+  const int n = p.hi > start ? (int)(((int64_t)p.hi - start + a.chunk - 1) / a.chunk) : 1;
+  p.splits = n < a.splits ? n : a.splits;
+}
+
+// The tile of a slot; false if it has none.
+__host__ __device__ inline bool place_of_slot(const AttentionArgs& a, int group, int slot, Place& p) {
+  const CacheArgs& c = a.c;
+  if (c.starts) {
+    int lo = 0, hi = c.batch + 1;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (first_slot(a, group, mid) <= slot) lo = mid; else hi = mid;
+    }
+    p.b = lo;
+    p.row0 = c.starts[lo];
+    const int next = lo < c.batch ? c.starts[lo + 1] : c.rows;
+    if (p.row0 < 0 || next <= p.row0 || next > c.rows) return false;
+    p.count = next - p.row0;
+    const int64_t tile = slot - first_slot(a, group, lo);
+    if (tile < 0 || tile * a.row_tile >= (int64_t)p.count * group) return false;
+    p.tile = (int)tile;
+  } else {
+    const int per = (group + a.row_tile - 1) / a.row_tile;
+    p.b = p.row0 = slot / per;
+    p.tile = slot - p.b * per;
+    p.count = 1;
+  }
+  if (p.b == c.batch && !a.fill_tail) return false;
+  fill_place(a, group, p);
+  return true;
+}
+
+// The tile of a query row and head, the slot it had and its row in the tile;
+// false if no sequence has the row.
+__host__ __device__ inline bool place_of_row(const AttentionArgs& a, int group, int row, int head, Place& p,
+                                             int64_t& slot, int& index) {
+  const CacheArgs& c = a.c;
+  if (c.starts) {
+    int lo = 0, hi = c.batch;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (c.starts[mid] <= row) lo = mid; else hi = mid;
+    }
+    p.b = lo;
+    p.row0 = c.starts[lo];
+    const int next = c.starts[lo + 1];
+    if (p.row0 < 0 || row < p.row0 || row >= next || next > c.rows) return false;
+    p.count = next - p.row0;
+    slot = first_slot(a, group, lo);
+  } else {
+    p.b = p.row0 = row;
+    p.count = 1;
+    slot = (int64_t)row * ((group + a.row_tile - 1) / a.row_tile);
+  }
+  const int local = (row - p.row0) * group + head % group;
+  p.tile = local / a.row_tile;
+  index = local - p.tile * a.row_tile;
+  slot += p.tile;
+  fill_place(a, group, p);
+  return true;
+}
+
+// ---- append ----------------------------------------------------------------
+
+// A page that gets tokens: its slots [from, to) get rows src, src + 1, ...
+struct PageWrite {
+  int pid, from, to, src;
+};
+
+// Slots of sequence b start at starts[b] / page + 2 b.
+__host__ __device__ inline int64_t append_slots(const CacheArgs& c) {
+  return c.starts ? (int64_t)c.rows / c.page + 2 * (int64_t)c.batch : c.batch;
+}
+
+__host__ __device__ inline bool page_of_slot(const CacheArgs& c, int slot, PageWrite& w) {
+  int b, row0, count, nth;
+  if (c.starts) {
+    int lo = 0, hi = c.batch;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (c.starts[mid] / c.page + 2 * mid <= slot) lo = mid; else hi = mid;
+    }
+    b = lo;
+    row0 = c.starts[b];
+    const int next = c.starts[b + 1];
+    if (row0 < 0 || next <= row0 || next > c.rows) return false;
+    count = next - row0;
+    nth = slot - (row0 / c.page + 2 * b);
+    if (nth < 0) return false;
+  } else {
+    b = row0 = slot;
+    count = 1;
+    nth = 0;
+  }
+  const int len = c.lens[b];
+  if (len <= 0) return false;
+  const int first = len - count;  // position of the first new token
+  const int begin = first > 0 ? first : 0;
+  const int block = begin / c.page + nth;
+  if (block > (len - 1) / c.page || block >= c.blocks) return false;
+  w.pid = c.table[b * c.ldt + block];
+  if (w.pid < 0 || w.pid >= c.pages) return false;
+  const int base = block * c.page;
+  w.from = begin > base ? begin - base : 0;
+  w.to = len - base < c.page ? len - base : c.page;
+  w.src = row0 + base + w.from - first;
+  return true;
+}
+
+}  // namespace serving

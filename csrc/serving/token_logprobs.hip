@@ -1,0 +1,328 @@
+// Of each row of logits x and its given token t: log p(t), the entropy of p,
+// the number of tokens above t, and the top alternatives, p = softmax(x).
+//
+// Bound by one read of the logits. A wave takes a span of consecutive logits
+// in registers, finds their largest m, and then, with u = (x - m) log2 e, sums
+// 2^u and 2^u u and counts x > x_t. (The difference comes first: x log2 e alone
+// would leave fp32's range where a mask is the type's lowest value.) On the way it leaves the largest of each 64 consecutive logits (one
+// 128-byte line of 16-bit ones): no other trace of the alternatives is needed,
+// since the k best logits, by value and then by lower index, lie in the k best
+// spans by their largest and then by lower index, and in these in the k best
+// groups of 64. A second launch joins a row's spans in a fixed order and reads
+// only those groups again.
+//
+// Sums are fp32 over at most 4096 values a span, 64 a lane.
+#include "device.h"
+#include "serving.h"
+
+namespace serving {
+namespace {
+
+constexpr int kUnits = 8;  // 16-byte loads of a lane
+
+template <typename T>
+struct Shape {
+  static constexpr int kVec = 16 / (int)sizeof(T);      // values of a load
+  static constexpr int kSpan = kUnits * 64 * kVec;      // of a wave
+  static constexpr int kGroups = kSpan / 64;
+  static constexpr int kLanes = 64 / kVec;              // lanes of a group
+};
+
+// Workspace of a row: per span {reference, sum, weighted sum, count}, then
+// the spans' largest, then the groups' largest.
+struct Layout {
+  int spans, groups;
+  int64_t row;  // floats of a row
+  __host__ __device__ Layout(int vocab, int span) {
+    spans = (vocab + span - 1 + 7) / span;  // a row may start within a 16-byte line
+    groups = span / 64;
+    row = (int64_t)spans * (5 + groups);
+  }
+  __device__ float* stats(float* w, int64_t r, int s) const { return w + r * row + s * 4; }
+  __device__ float* tops(float* w, int64_t r) const { return w + r * row + spans * 4; }
+  __device__ float* group(float* w, int64_t r, int s) const { return w + r * row + spans * 5 + (int64_t)s * groups; }
+};
+
+__device__ __forceinline__ void unpack(u32x4 v, float* f, const __bf16*) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = bits_as<float>(v[i] << 16);
+    f[2 * i + 1] = bits_as<float>(v[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void unpack(u32x4 v, float* f, const _Float16*) {
+  const f16x8 h = bits_as<f16x8>(v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = (float)h[i];
+}
+__device__ __forceinline__ void unpack(u32x4 v, float* f, const float*) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = bits_as<float>(v[i]);
+}
+
+// Larger of a lane's and its neighbour's; NaN gives way.
+__device__ __forceinline__ float max_xor(float v, int mask) { return fmaxf(v, __shfl_xor(v, mask)); }
+
+// Whole numbers in the order of the values: -0 equals 0, NaN is above all.
+__device__ __forceinline__ uint32_t order_of(float f) {
+  if (f != f) return 0xFFFFFFFFu;
+  const uint32_t b = bits_as<uint32_t>(f + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void spans_kernel(LogprobArgs a) {
+  using S = Shape<T>;
+  constexpr int V = S::kVec;
+  const Layout lay(a.vocab, S::kSpan);
+  const int lane = threadIdx.x & 63;
+  const int span = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (span >= lay.spans) return;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const T* x = (const T*)a.logits + row * a.ld;
+    const int shift = (int)(((uintptr_t)x / sizeof(T)) % V);
+    const int first = span * S::kSpan + lane * V - shift;  // index of the lane's first value
+
+    u32x4 raw[kUnits];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int e = first + u * 64 * V;
+      if (e >= 0 && e + V <= a.vocab) {
+        raw[u] = *reinterpret_cast<const u32x4*>(x + e);
+      } else {  // the row's ends: nothing outside it is read
+        T part[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) part[i] = (e + i >= 0 && e + i < a.vocab) ? x[e + i] : (T)-kInf;
+        __builtin_memcpy(&raw[u], part, 16);
+      }
+    }
+    const int64_t t = a.targets[row];
+    const bool known = t >= 0 && t < a.vocab;
+    const float xt = known ? (float)x[t] : kInf;
+
+    float best[kUnits];  // of the lane's group of 64 values
+    float m = -kInf;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      float f[V];
+      unpack(raw[u], f, (const T*)nullptr);
+      float b = f[0];
+#pragma unroll
+      for (int i = 1; i < V; ++i) b = fmaxf(b, f[i]);
+#pragma unroll
+      for (int d = 1; d < S::kLanes; d <<= 1) b = max_xor(b, d);
+      best[u] = b;
+      m = fmaxf(m, b);
+    }
+#pragma unroll
+    for (int d = S::kLanes; d < 64; d <<= 1) m = max_xor(m, d);
+
+    const float ref = m == -kInf ? 0.f : m;
+    float sum = 0.f, weighted = 0.f;
+    int above = 0;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      float f[V];
+      unpack(raw[u], f, (const T*)nullptr);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float d = (f[i] - ref) * kLog2e;
+        const float p = __builtin_amdgcn_exp2f(d);
+        sum += p;
+        weighted = __builtin_fmaf(p, fmaxf(d, -256.f), weighted);  // 2^-256 is 0: no 0 x inf
+        above += __popcll(__ballot(f[i] > xt));
+      }
+    }
+    const bool odd = __any(sum != sum);  // a NaN or an infinity among the values
+    if (odd) {
+      float top = -kInf;
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        float f[V];
+        unpack(raw[u], f, (const T*)nullptr);
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < V; ++i) nan |= f[i] != f[i];
+        int any = nan;
+#pragma unroll
+        for (int d = 1; d < S::kLanes; d <<= 1) any |= __shfl_xor(any, d);
+        if (any) best[u] = __builtin_nanf("");
+        if (__any(nan)) top = __builtin_nanf("");
+      }
+      if (top != top) m = top;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      sum += __shfl_xor(sum, d);
+      weighted += __shfl_xor(weighted, d);
+    }
+    if (lane == 0) {
+      f32x4 s;
+      s[0] = m == -kInf ? -kInf : ref;
+      s[1] = sum;
+      s[2] = weighted;
+      s[3] = bits_as<float>(above);
+      float* to = lay.stats(a.work, row, span);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) to[i] = s[i];
+      lay.tops(a.work, row)[span] = m;
+    }
+    if (a.top && lane % S::kLanes == 0) {
+      float* to = lay.group(a.work, row, span) + lane / S::kLanes;
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) to[u * (64 / S::kLanes)] = best[u];
+    }
+  }
+}
+
+// Lists of (order, place) in LDS, one list a wave; a key is larger where the
+// value is, and among equal values where the place is lower. A list holds the
+// spans, then at most 64 members of each of `top` parts.
+inline int list_size(int spans, int top) { return top == 0 ? 0 : spans > 64 * top ? spans : 64 * top; }
+
+__device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t place) {
+  return (uint64_t)order << 32 | (uint32_t)~place;
+}
+
+// Sorts out the `want` largest of list[0..n), all different, into out[0..want)
+// in falling order. The wave works alone.
+__device__ void select_top(const uint64_t* list, int n, int want, uint64_t* out, int lane) {
+  uint64_t floor_key = 0;  // keys from here on are the `want` largest
+  if (n > 256 && n > want) {
+    // the want-th largest by its bits, from the top: exact, for any list
+    for (int bit = 63; bit >= 0; --bit) {
+      const uint64_t trial = floor_key | 1ull << bit;
+      int count = 0;
+      for (int i = lane; i < n; i += 64) count += list[i] >= trial;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) count += __shfl_xor(count, d);
+      if (count >= want) floor_key = trial;
+    }
+  }
+  for (int i = lane; i < n; i += 64) {
+    const uint64_t key = list[i];
+    if (key < floor_key) continue;
+    int place = 0;
+    for (int j = 0; j < n; ++j) place += list[j] > key;
+    if (place < want) out[place] = key;
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(64) void rows_kernel(LogprobArgs a) {
+  using S = Shape<T>;
+  const Layout lay(a.vocab, S::kSpan);
+  const int lane = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  const T* x = (const T*)a.logits + row * a.ld;
+  const int64_t t = a.targets[row];
+  const bool known = t >= 0 && t < a.vocab;
+
+  // the spans' sums against one reference, each lane's in the spans' order
+  const float* stats = lay.stats(a.work, row, 0);
+  float ref = -kInf;
+  for (int s = lane; s < lay.spans; s += 64) ref = fmaxf(ref, stats[s * 4]);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) ref = max_xor(ref, d);
+  float sum = 0.f, weighted = 0.f;
+  int64_t above = 0;
+  for (int s = lane; s < lay.spans; s += 64) {
+    const float r = stats[s * 4], q = stats[s * 4 + 1], w = stats[s * 4 + 2];
+    above += bits_as<int>(stats[s * 4 + 3]);
+    if (r == -kInf && !(q != q)) continue;  // nothing allowed in this span
+    const float d = (r - ref) * kLog2e;
+    const float f = __builtin_amdgcn_exp2f(d);
+    sum += q * f;
+    weighted += f * __builtin_fmaf(q, d < -256.f ? -256.f : d, w);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    sum += __shfl_xor(sum, d);
+    weighted += __shfl_xor(weighted, d);
+    above += __shfl_xor(above, d);
+  }
+  const float log_sum = __builtin_amdgcn_logf(sum) * kLn2;
+  const bool empty = ref == -kInf && !(sum != sum);  // every token masked
+  auto logp = [&](float v) { return empty ? -kInf : (v - ref) - log_sum; };
+  if (lane == 0) {
+    a.logprob[row] = known ? logp((float)x[t]) : t < 0 ? 0.f : __builtin_nanf("");
+    a.entropy[row] = empty ? 0.f : log_sum - weighted / sum * kLn2;
+    a.rank[row] = known ? above : -1;
+  }
+  if (a.top == 0) return;
+
+  extern __shared__ uint64_t list[];  // list_size()
+  __shared__ uint64_t out[3][kMaxTop];
+  const int want = a.top;
+  const int shift = (int)(((uintptr_t)x / sizeof(T)) % S::kVec);
+  const float* tops = lay.tops(a.work, row);
+
+  // spans, then groups of 64, then logits
+  int n = lay.spans;
+  for (int i = lane; i < n; i += 64) list[i] = key_of(order_of(tops[i]), i);
+  __syncthreads();
+  int got = n < want ? n : want;
+  select_top(list, n, got, out[0], lane);
+  __syncthreads();
+#pragma unroll 1
+  for (int level = 1; level <= 2; ++level) {
+    // members of the last level's parts; those under its least are left out
+    const int parts = got;
+    const int size = level == 1 ? S::kGroups : 64;
+    const uint32_t least = parts == want ? (uint32_t)(out[level - 1][parts - 1] >> 32) : 0u;
+    n = 0;
+    for (int p = 0; p < parts; ++p) {
+      const uint32_t part = ~(uint32_t)out[level - 1][p];
+      uint32_t order = 0;
+      uint32_t place = part * size + lane;
+      bool in = lane < size;
+      if (level == 1) {
+        if (in) order = order_of(lay.group(a.work, row, 0)[place]);
+      } else {
+        const int e = (int)place - shift;
+        in = e >= 0 && e < a.vocab;
+        place = (uint32_t)e;
+        if (in) order = order_of((float)x[e]);
+      }
+      in = in && order >= least;
+      const uint64_t mask = __ballot(in);
+      if (in) list[n + __popcll(mask & ((1ull << lane) - 1))] = key_of(order, place);
+      n += __popcll(mask);
+    }
+    __syncthreads();
+    got = n < want ? n : want;
+    select_top(list, n, got, out[level], lane);
+    __syncthreads();
+  }
+  for (int i = lane; i < want; i += 64) {
+    const uint32_t id = ~(uint32_t)out[2][i];
+    a.top_ids[row * want + i] = id;
+    a.top_logprobs[row * want + i] = logp((float)x[id]);
+  }
+}
+
+template <typename T>
+hipError_t launch(const LogprobArgs& a, hipStream_t stream) {
+  const Layout lay(a.vocab, Shape<T>::kSpan);
+  const dim3 grid((lay.spans + 3) / 4, a.rows < 65535 ? (int)a.rows : 65535);
+  spans_kernel<T><<<grid, 256, 0, stream>>>(a);
+  if (hipError_t e = hipGetLastError()) return e;
+  const size_t lds = sizeof(uint64_t) * list_size(lay.spans, a.top);
+  rows_kernel<T><<<dim3((unsigned)a.rows), 64, lds, stream>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t logprob_workspace(int64_t rows, int vocab, int dtype) {
+  const int span = dtype == kF32 ? Shape<float>::kSpan : Shape<__bf16>::kSpan;
+  return rows * Layout(vocab, span).row;
+}
+
+hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t stream) {
+  if (a.dtype == kBF16) return launch<__bf16>(a, stream);
+  if (a.dtype == kF16) return launch<_Float16>(a, stream);
+  return launch<float>(a, stream);
+}
+
+}  // namespace serving

@@ -1,0 +1,294 @@
+"""The serving-step operators on the host: layouts, work partition, refusals.
+
+The partition of work (which workgroup has which rows, tokens and pages) is
+plain arithmetic that the kernels share with host checks, so that lengths,
+starts and page tables of every kind, broken ones too, are tried here.
+"""
+
+import random
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytest.importorskip("gpud_amd.diag._serving", reason="native extension not built")
+
+from gpud_amd.diag import _serving, serving  # noqa: E402
+
+BF16, FP16, F8 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
+
+
+# -- layouts -----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n,k,group", [(1, 1, 32), (16, 128, 128), (17, 129, 64), (40, 300, 32), (100, 513, 128)])
+def test_pack_w4_keeps_every_code_in_its_documented_place(n, k, group):
+    g = torch.Generator().manual_seed(n * k)
+    codes = torch.randint(0, 16, (n, k), generator=g)
+    groups = -(-k // group)
+    scales = torch.rand(n, groups, generator=g).to(BF16)
+    zeros = torch.randint(0, 16, (n, groups), generator=g)
+    packed, s, z = serving.pack_w4(codes, scales, zeros, group_size=group)
+    assert packed.shape == (-(-n // 16), -(-k // 128), 64, 16) and packed.is_contiguous()
+    assert torch.equal(serving.unpack_w4(packed, n, k), codes.to(torch.uint8))
+    rng = random.Random(k)
+    for _ in range(200):
+        row, col = rng.randrange(n), rng.randrange(k)
+        b, c = divmod(col, 128)
+        j, lanes, e = c // 32, c % 32 // 8, c % 8
+        nibble = e // 2 + 4 * (e % 2)
+        byte = int(packed[row // 16, b, 16 * lanes + row % 16, 4 * j + nibble // 2])
+        assert byte >> 4 * (nibble % 2) & 15 == int(codes[row, col])
+        assert s[row // 16, col // group, row % 16] == scales[row, col // group]
+        assert z[row // 16, col // group, row % 16] == zeros[row, col // group]
+
+
+def test_pack_w4_refuses_what_does_not_fit():
+    codes, scales = torch.zeros(16, 128, dtype=torch.long), torch.ones(16, 1, dtype=BF16)
+    for bad in (codes + 16, codes - 1):
+        with pytest.raises(ValueError, match="0..15"):
+            serving.pack_w4(bad, scales)
+    with pytest.raises(ValueError, match="group_size"):
+        serving.pack_w4(codes, scales, group_size=16)
+    with pytest.raises(ValueError, match="scales"):
+        serving.pack_w4(codes, scales, group_size=64)
+    with pytest.raises(ValueError, match="zeros"):
+        serving.pack_w4(codes, scales, torch.zeros(16, 2))
+    with pytest.raises(ValueError, match="whole numbers"):
+        serving.pack_w4(codes.float(), scales)
+    with pytest.raises(ValueError, match="empty"):
+        serving.pack_w4(codes[:0], scales[:0])
+
+
+def test_cache_scale_is_the_smallest_power_of_two_that_fits():
+    amax = torch.tensor([0.0, 1e-30, 1.0, 448.0, 448.1, 449.0, 3.5, 3.5001, 7.0, 1e30, 2.0**-64 * 448])
+    got = serving.cache_scale(amax)
+    assert torch.equal(torch.frexp(got).mantissa, torch.full_like(got, 0.5))
+    assert bool((amax <= 448 * got).all())
+    assert bool(((amax > 224 * got) | (got == 2.0**-64)).all())
+
+
+# -- partition ---------------------------------------------------------------
+
+
+def _random_batch(rng):
+    batch = rng.choice([1, 2, 3, 7, 20])
+    counts = [rng.choice([0, 1, 1, 2, 5, 33, 200]) for _ in range(batch)]
+    starts = [0]
+    for n in counts:
+        starts.append(starts[-1] + n)
+    lens = [max(0, n + rng.choice([-3, 0, 0, 1, 63, 64, 300, 900])) for n in counts]
+    return starts, lens
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_attention_gives_each_row_its_tokens_once(seed):
+    rng = random.Random(seed)
+    starts, lens = _random_batch(rng)
+    group, heads = rng.choice([1, 3, 4, 8, 16, 40]), 2
+    tail = rng.choice([0, 1, 50])
+    rows = starts[-1] + tail
+    if not rows:
+        return
+    page, blocks, window = rng.choice([16, 64]), 80, rng.choice([0, 1, 64, 100])
+    fill = rng.random() < 0.5
+    got = _serving.attention_places(starts, lens, rows, heads, heads * group, page, blocks, window, rng.choice([1, 700, 5000]), fill)
+    spans = {}
+    for row, head, slot, split, lo, hi in got:
+        spans.setdefault((row, head), []).append((split, lo, hi))
+    want = rows if fill else starts[-1]
+    assert set(spans) == {(r, h) for r in range(want) for h in range(group)}
+    for b, length in enumerate(lens):
+        count = starts[b + 1] - starts[b]
+        for i in range(count):
+            pos = length - count + i
+            for h in range(group):
+                parts = sorted(spans[starts[b] + i, h])
+                assert [p[0] for p in parts] == list(range(len(parts)))
+                for p, q in zip(parts, parts[1:]):
+                    assert p[2] == q[1] and p[2] % 64 == 0
+                lo = max(0, pos - window + 1) if window else 0
+                assert parts[0][1] <= lo and parts[-1][2] > pos if pos >= 0 else True
+                assert parts[-1][2] <= max(length, 0)
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_attention_survives_any_starts_and_lengths(seed):
+    """Broken metadata may leave rows out; it never names a row that is not there."""
+    rng = random.Random(seed)
+    batch, rows = rng.choice([1, 4]), 50
+    wild = lambda: rng.choice([-(2**31), -5, 0, 3, 49, 50, 51, 60, 10**6])  # noqa: E731
+    starts = [wild() for _ in range(batch + 1)]
+    lens = [rng.choice([-(2**31), -1, 0, 5, 64, 10**6, 2**31 - 1]) for _ in range(batch)]
+    for row, head, slot, split, lo, hi in _serving.attention_places(starts, lens, rows, 2, 8, 16, 8, rng.choice([0, 5]), 100, True):
+        assert 0 <= row < rows and 0 <= head < 4 and 0 <= lo and hi <= 128
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_append_gives_each_new_token_its_slot_once(seed):
+    rng = random.Random(seed)
+    starts, lens = _random_batch(rng)
+    page, blocks = rng.choice([16, 64]), 80
+    rows = starts[-1] + rng.choice([0, 9])
+    batch = len(lens)
+    table = list(range(batch * blocks))
+    rng.shuffle(table)
+    got = {}
+    for slot, pid, lo, hi, src in _serving.append_places(starts, lens, table, rows, page, blocks, batch * blocks):
+        assert 0 <= lo < hi <= page
+        for i in range(lo, hi):
+            assert (pid, i) not in got
+            got[pid, i] = src + i - lo
+    want = {}
+    for b, length in enumerate(lens):
+        count = starts[b + 1] - starts[b]
+        for i in range(count):
+            pos = length - count + i
+            if pos >= 0:
+                want[table[b * blocks + pos // page], pos % page] = starts[b] + i
+    assert got == want
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_append_survives_any_metadata(seed):
+    rng = random.Random(seed)
+    batch, rows, blocks, page, pages = rng.choice([1, 4]), 50, 3, 16, 6
+    starts = [rng.choice([-(2**31), -5, 0, 3, 49, 50, 51, 10**6]) for _ in range(batch + 1)]
+    lens = [rng.choice([-(2**31), -1, 0, 5, 48, 49, 2**31 - 1]) for _ in range(batch)]
+    table = [rng.choice([-1, 0, 5, 6, 2**31 - 1]) for _ in range(batch * blocks)]
+    for slot, pid, lo, hi, src in _serving.append_places(starts, lens, table, rows, page, blocks, pages):
+        assert 0 <= pid < pages and 0 <= lo < hi <= page and 0 <= src and src + hi - lo <= rows
+
+
+# -- refusals ----------------------------------------------------------------
+
+
+def w4_args(**change):
+    a = dict(
+        x=torch.zeros(3, 256, dtype=BF16), codes=torch.zeros(2, 2, 64, 16, dtype=torch.uint8),
+        scales=torch.zeros(2, 2, 16, dtype=BF16), zeros=None, out_features=20, group_size=128,
+    )
+    a.update(change)
+    return a
+
+
+@pytest.mark.parametrize(
+    "change,error,match",
+    [
+        (dict(), ValueError, "on a GPU"),
+        (dict(x=[1.0]), TypeError, "tensor"),
+        (dict(x=torch.zeros(3, 256)), TypeError, "float32"),
+        (dict(x=torch.zeros(256, dtype=BF16)), ValueError, "2 dimensions"),
+        (dict(x=torch.zeros(3, 0, dtype=BF16)), ValueError, "no product"),
+        (dict(x=torch.zeros(3, 300, dtype=BF16)), ValueError, "codes has shape"),
+        (dict(out_features=0), ValueError, "no product"),
+        (dict(out_features=33), ValueError, "codes has shape"),
+        (dict(group_size=100), ValueError, "group_size"),
+        (dict(group_size=64), ValueError, "scales has shape"),
+        (dict(scales=torch.zeros(2, 2, 16, dtype=FP16)), TypeError, "scales"),
+        (dict(codes=torch.zeros(2, 2, 64, 32, dtype=torch.uint8)[..., ::2]), ValueError, "contiguous"),
+        (dict(zeros=torch.zeros(2, 2, 16)), TypeError, "zeros"),
+        (dict(zeros=torch.zeros(2, 1, 16, dtype=torch.uint8)), ValueError, "zeros has shape"),
+        (dict(out=torch.zeros(3, 20)), TypeError, "out"),
+        (dict(out=torch.zeros(3, 21, dtype=BF16)), ValueError, "out must be"),
+        (dict(out=torch.zeros(20, dtype=BF16).expand(3, 20)), ValueError, "overlap"),
+        (dict(x=torch.zeros(3, 256, dtype=BF16, requires_grad=True)), ValueError, "no backward"),
+    ],
+)
+def test_w4_matmul_refuses(change, error, match):
+    a = w4_args(**change)
+    with pytest.raises(error, match=match):
+        serving.w4_matmul(a.pop("x"), a.pop("codes"), a.pop("scales"), a.pop("zeros"), **a)
+
+
+def cache_args(**change):
+    a = dict(
+        k_cache=torch.zeros(5, 2, 16, 64).to(F8), v_cache=torch.zeros(5, 2, 64, 16).to(F8),
+        k_scale=torch.ones(5, 2), v_scale=torch.ones(5, 2), block_table=torch.zeros(3, 4, dtype=torch.int32),
+        seq_lens=torch.ones(3, dtype=torch.int32), query_start=None,
+    )
+    a.update(change)
+    return a
+
+
+BAD_CACHE = [
+    (dict(), ValueError, "on a GPU"),
+    (dict(k_cache=torch.zeros(5, 2, 16, 64)), TypeError, "k_cache"),
+    (dict(v_cache=torch.zeros(5, 2, 16, 64).to(F8)), ValueError, "v_cache has shape"),
+    (dict(k_cache=torch.zeros(5, 2, 24, 64).to(F8)), ValueError, "page size"),
+    (dict(k_cache=torch.zeros(5, 2, 16, 72).to(F8)), ValueError, "head dimension"),
+    (dict(k_cache=torch.zeros(5, 2, 16, 272).to(F8)), ValueError, "head dimension"),
+    (dict(k_cache=torch.zeros(0, 2, 16, 64).to(F8)), ValueError, "no cache"),
+    (dict(k_scale=torch.ones(5, 1)), ValueError, "k_scale has shape"),
+    (dict(v_scale=torch.ones(5, 2, dtype=BF16)), TypeError, "v_scale"),
+    (dict(block_table=torch.zeros(3, 4, dtype=torch.long)), TypeError, "block_table"),
+    (dict(block_table=torch.zeros(4, 3, dtype=torch.int32).t()), ValueError, "dense"),
+    (dict(seq_lens=torch.ones(2, dtype=torch.int32)), ValueError, "seq_lens has shape"),
+    (dict(seq_lens=torch.ones(3, dtype=torch.long)), TypeError, "seq_lens"),
+    (dict(query_start=torch.zeros(3, dtype=torch.int32)), ValueError, "query_start has shape"),
+    (dict(block_table=torch.zeros(2, 4, dtype=torch.int32), seq_lens=torch.ones(2, dtype=torch.int32)), ValueError, "query_start"),
+]
+
+
+@pytest.mark.parametrize("change,error,match", BAD_CACHE)
+def test_cache_append_refuses(change, error, match):
+    k = torch.zeros(3, 2, 64, dtype=BF16)
+    with pytest.raises(error, match=match):
+        serving.cache_append(k, k, **cache_args(**change))
+
+
+def test_cache_append_refuses_new_tokens_that_do_not_fit():
+    k = torch.zeros(3, 2, 64, dtype=BF16)
+    for bad, error in ((k.float(), TypeError), (k[:, :1], ValueError), (k[0], ValueError), (k.half(), TypeError)):
+        with pytest.raises(error):
+            serving.cache_append(k, bad, **cache_args())
+
+
+@pytest.mark.parametrize("change,error,match", BAD_CACHE)
+def test_cache_attention_refuses(change, error, match):
+    with pytest.raises(error, match=match):
+        serving.cache_attention(torch.zeros(3, 4, 64, dtype=BF16), **cache_args(**change))
+
+
+@pytest.mark.parametrize(
+    "q,more,error,match",
+    [
+        (torch.zeros(3, 4, 64), {}, TypeError, "q has type"),
+        (torch.zeros(3, 3, 64, dtype=BF16), {}, ValueError, "evenly"),
+        (torch.zeros(3, 0, 64, dtype=BF16), {}, ValueError, "evenly"),
+        (torch.zeros(3, 4, 80, dtype=BF16), {}, ValueError, "head dimension 80"),
+        (torch.zeros(3, 4, 64, dtype=BF16), dict(window=0), ValueError, "window"),
+        (torch.zeros(3, 4, 64, dtype=BF16), dict(scale=float("inf")), ValueError, "scale"),
+        (torch.zeros(3, 4, 64, dtype=BF16), dict(out=torch.zeros(3, 4, 64)), TypeError, "out"),
+        (torch.zeros(3, 4, 64, dtype=BF16), dict(out=torch.zeros(3, 64, 4, dtype=BF16).transpose(1, 2)), ValueError, "contiguous"),
+        (torch.zeros(3, 4, 64, dtype=BF16, requires_grad=True), {}, ValueError, "no backward"),
+    ],
+)
+def test_cache_attention_refuses_queries(q, more, error, match):
+    with pytest.raises(error, match=match):
+        serving.cache_attention(q, **cache_args(), **more)
+
+
+@pytest.mark.parametrize(
+    "logits,targets,top,error,match",
+    [
+        (torch.zeros(2, 9), torch.zeros(2, dtype=torch.long), 3, ValueError, "on a GPU"),
+        (torch.zeros(2, 9).double(), torch.zeros(2, dtype=torch.long), 0, TypeError, "float64"),
+        (torch.zeros(9), torch.zeros(1, dtype=torch.long), 0, ValueError, "2 dimensions"),
+        (torch.zeros(2, 9), torch.zeros(2, dtype=torch.int32), 0, TypeError, "targets"),
+        (torch.zeros(2, 9), torch.zeros(3, dtype=torch.long), 0, ValueError, "3 targets"),
+        (torch.zeros(2, 9), torch.zeros(2, dtype=torch.long), 10, ValueError, "top_k"),
+        (torch.zeros(2, 99), torch.zeros(2, dtype=torch.long), 65, ValueError, "top_k"),
+        (torch.zeros(2, 9), torch.zeros(2, dtype=torch.long), -1, ValueError, "top_k"),
+        (torch.zeros(2, 0), torch.zeros(2, dtype=torch.long), 0, ValueError, "vocabulary"),
+        (torch.zeros(1, 1).expand(1, 2**22 + 1), torch.zeros(1, dtype=torch.long), 0, ValueError, "vocabulary"),
+    ],
+)
+def test_token_logprobs_refuses(logits, targets, top, error, match):
+    with pytest.raises(error, match=match):
+        serving.token_logprobs(logits, targets, top)
+
+
+def test_new_cache_refuses_sizes():
+    for bad in ((0, 1, 64, 16), (1, 0, 64, 16), (1, 1, 65, 16), (1, 1, 64, 20), (1, 1, 64, 8)):
+        with pytest.raises(ValueError):
+            serving.new_cache(*bad, device="cpu")

@@ -45,7 +45,7 @@ fi
 
 if [ -f csrc/diag/fabric_rccl.cpp ]; then
   echo "[build] rccl fabric check binary"
-  ${ROCM}/bin/hipcc ${HIPFLAGS} -O2 \
+  ${ROCM}/bin/hipcc --offload-arch=gfx950 -O2 -std=c++17 \
       -I${ROCM}/include csrc/diag/fabric_rccl.cpp \
       -L${ROCM}/lib -lrccl -Wl,-rpath,${ROCM}/lib \
       -o gpud_amd/diag/gpud-fabric-check

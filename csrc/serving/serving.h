@@ -23,7 +23,11 @@ struct W4Args {
   int64_t ldx, ldy;
   int m, n, k, group;     // group: 32, 64 or 128
   int dtype;              // kBF16 or kF16
+  void* work;             // w4_workspace() bytes, or null if 0
 };
+int64_t w4_workspace(const W4Args& a);
+// Largest K: its scales and zero points have to fit the LDS.
+constexpr int kMaxColumns = 32768;
 hipError_t launch_w4_matmul(const W4Args& a, hipStream_t stream);
 
 // ---- 8-bit paged cache ----------------------------------------------------

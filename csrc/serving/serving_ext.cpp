@@ -50,21 +50,31 @@ class OnDevice {
 
 hipStream_t stream_of(uintptr_t s) { return reinterpret_cast<hipStream_t>(s); }
 
-void w4_matmul(int device, uintptr_t stream, uintptr_t x, int64_t ldx, uintptr_t codes, uintptr_t scales,
-               uintptr_t zeros, uintptr_t y, int64_t ldy, int m, int n, int k, int group, int dtype) {
+W4Args w4_args(uintptr_t x, int64_t ldx, int m, int n, int k, int group, int dtype) {
   W4Args a{};
   a.x = ptr<void>(x);
   a.ldx = ldx;
-  a.codes = ptr<uint8_t>(codes);
-  a.scales = ptr<void>(scales);
-  a.zeros = ptr<uint8_t>(zeros);
-  a.y = ptr<void>(y);
-  a.ldy = ldy;
   a.m = m;
   a.n = n;
   a.k = k;
   a.group = group;
   a.dtype = dtype;
+  return a;
+}
+
+int64_t w4_work(uintptr_t x, int64_t ldx, int m, int n, int k, int group, int dtype) {
+  return w4_workspace(w4_args(x, ldx, m, n, k, group, dtype));
+}
+
+void w4_matmul(int device, uintptr_t stream, uintptr_t x, int64_t ldx, int m, int n, int k, int group, int dtype,
+               uintptr_t codes, uintptr_t scales, uintptr_t zeros, uintptr_t y, int64_t ldy, uintptr_t work) {
+  W4Args a = w4_args(x, ldx, m, n, k, group, dtype);
+  a.codes = ptr<uint8_t>(codes);
+  a.scales = ptr<void>(scales);
+  a.zeros = ptr<uint8_t>(zeros);
+  a.y = ptr<void>(y);
+  a.ldy = ldy;
+  a.work = ptr<void>(work);
   OnDevice on(device);
   OnDevice::check(launch_w4_matmul(a, stream_of(stream)), "w4_matmul");
 }
@@ -238,6 +248,7 @@ std::vector<std::vector<int64_t>> append_places(const std::vector<int32_t>& star
 
 PYBIND11_MODULE(_serving, m) {
   m.doc() = "gpud_amd CDNA4 serving-step operators (4-bit products, 8-bit cache, token log probabilities)";
+  m.def("w4_workspace", &w4_work);
   m.def("w4_matmul", &w4_matmul);
   m.def("cache_append", &cache_append);
   m.def("attention_plan", &attention_plan);
@@ -246,6 +257,7 @@ PYBIND11_MODULE(_serving, m) {
   m.def("attention_places", &attention_places);
   m.def("append_places", &append_places);
   m.def("token_logprobs", &token_logprobs);
+  m.attr("MAX_COLUMNS") = kMaxColumns;
   m.attr("MAX_TOP") = kMaxTop;
   m.attr("MAX_VOCAB") = kMaxVocab;
 }

@@ -7,43 +7,61 @@
 // operand, so that up to 16 tokens ride along as columns at no further cost.
 //
 // A nibble q becomes the operand's type by putting it into the top mantissa
-// bits of 16.0: 16 + q exactly, for bf16 and fp16 alike, two codes an
-// instruction pair. A second product with the constant -(16 + z) takes the
-// offset off again inside the fp32 accumulator, so each product is of x with
-// a whole number of at most 5 bits and nothing is rounded before the sum. A
-// group's scale multiplies its fp32 sum.
+// bits of 16.0: 16 + q exactly, for bf16 and fp16 alike, two codes in two
+// instructions. A second product with a constant takes the offset (and the
+// zero point, where all are 8) off again inside the fp32 accumulator; it is one
+// for all weight rows and gives the sum of x that zero points are times. Each
+// product is of x with a whole number of at most 5 bits, and nothing is rounded
+// before the fp32 sum of a group, which its scale multiplies.
 //
-// The waves of a workgroup split the columns and join their sums in LDS, in
+// The 8 waves of a workgroup split the columns and join their sums in LDS, in
 // the waves' order, so that results do not depend on timing.
+//
+// What the tokens cost beside the codes decides the rest (us, measured):
+// - Every load occupies the address path for 16 cycles, however little it
+//   fetches, as long as a load of 1 KB of codes. So scales and zero points come
+//   through LDS, and tokens too while they are under 32 KB in all: 1 x 28672 x
+//   8192 takes 24 with them in LDS, 29 without.
+// - Tokens that do not fit are read by every workgroup through the L2, so more
+//   than one tile of rows shares them where enough workgroups are left for the
+//   256 compute units: 4 tiles from 1024 on (64 x 16384 x 8192: 30, with two 37),
+//   2 from 512 on (5 x 8192 x 8192: 10.4; with one 11.3, with four 14.0), else 1
+//   (16 x 4096 x 4096: 7.7; with two 8.1).
+// - Rows of tokens a power of two apart fall on the same channels of the L2. A
+//   launch before lays tokens out in the order of the loads, which pays from two
+//   tiles of tokens on (64 x 16384 x 8192: 30 + 2.5, against 45), but not for one
+//   (16 x 28672 x 8192: 28.5 + 2.5, against 30). It also takes rows that 16-byte
+//   loads do not fit.
+// - The codes pass by the L2 (non-temporal): 5% at the largest sizes.
 #include "device.h"
 #include "serving.h"
 
 namespace serving {
 namespace {
 
-// 8 codes of a dword in the order of 8 consecutive columns, plus 16 each.
+// 8 codes of a dword in the order of 8 consecutive columns, plus 16 each. The
+// instruction that masks and sets bits takes no constants: its mask lives in a
+// vector register and its base in a scalar one, made once.
 template <typename T>
-__device__ __forceinline__ typename Mat<T>::x8 decode8(uint32_t w);
-
-template <>
-__device__ __forceinline__ bf16x8 decode8<__bf16>(uint32_t w) {
-  u32x4 r;
-  r[0] = ((w << 3) & 0x00780078u) | 0x41804180u;
-  r[1] = ((w >> 1) & 0x00780078u) | 0x41804180u;
-  r[2] = ((w >> 5) & 0x00780078u) | 0x41804180u;
-  r[3] = ((w >> 9) & 0x00780078u) | 0x41804180u;
-  return bits_as<bf16x8>(r);
-}
-
-template <>
-__device__ __forceinline__ f16x8 decode8<_Float16>(uint32_t w) {
-  u32x4 r;
-  r[0] = ((w << 6) & 0x03C003C0u) | 0x4C004C00u;
-  r[1] = ((w << 2) & 0x03C003C0u) | 0x4C004C00u;
-  r[2] = ((w >> 2) & 0x03C003C0u) | 0x4C004C00u;
-  r[3] = ((w >> 6) & 0x03C003C0u) | 0x4C004C00u;
-  return bits_as<f16x8>(r);
-}
+struct Decoder {
+  static constexpr bool kHalf = __is_same(T, _Float16);
+  static constexpr int kTop = kHalf ? 6 : 3;  // lowest of the 4 bits in a half dword
+  uint32_t mask = kHalf ? 0x03C003C0u : 0x00780078u;
+  uint32_t base = kHalf ? 0x4C004C00u : 0x41804180u;
+  __device__ __forceinline__ Decoder() {
+    asm("" : "+v"(mask));
+    asm("" : "+s"(base));
+  }
+  __device__ __forceinline__ typename Mat<T>::x8 operator()(uint32_t w) const {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int up = kTop - 4 * i;
+      r[i] = ((up >= 0 ? w << (up & 31) : w >> (-up & 31)) & mask) | base;
+    }
+    return bits_as<typename Mat<T>::x8>(r);
+  }
+};
 
 template <typename T>
 __device__ __forceinline__ typename Mat<T>::x8 splat8(float v) {
@@ -53,120 +71,214 @@ __device__ __forceinline__ typename Mat<T>::x8 splat8(float v) {
   return r;
 }
 
-// 8 values of row `x` from column k on; columns past the last are 0.
-template <typename T, bool kVec>
-__device__ __forceinline__ typename Mat<T>::x8 load_x8(const T* x, int k, int cols, bool live) {
-  typename Mat<T>::x8 r = bits_as<typename Mat<T>::x8>(u32x4{0, 0, 0, 0});
-  if constexpr (kVec) {
-    if (live && k < cols) r = *reinterpret_cast<const typename Mat<T>::x8*>(x + k);
-  } else {
-    if (live) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (k + i < cols) r[i] = x[k + i];
-    }
+// LDS of a workgroup: scales and zero points of its tiles, then the tokens if
+// they are few; the waves' sums take its place at the end.
+template <typename T, int MT, int NT>
+struct Lds {
+  int groups, scales, zeros, x, pitch;  // bytes, and elements of a token's row
+  size_t size;
+  __host__ __device__ Lds(const W4Args& a, bool with_x, int waves) {
+    groups = (a.k + a.group - 1) / a.group;
+    scales = NT * groups * 16 * (int)sizeof(T);
+    zeros = a.zeros ? NT * groups * 16 : 0;
+    // 16 bytes more than whole blocks: rows start in different banks
+    pitch = (a.k + 127) / 128 * 128 + 8;
+    x = with_x ? (a.m < 16 * MT ? a.m : 16 * MT) * pitch * (int)sizeof(T) : 0;
+    size = (size_t)scales + zeros + x;
+    const size_t sums = (size_t)waves * NT * MT * 1024;
+    if (size < sums) size = sums;
   }
-  return r;
-}
+};
 
-// MT tiles of 16 tokens, NT tiles of 16 weight rows, groups of G columns.
-template <typename T, int MT, int NT, int G, bool kZeros, bool kVec, int W>
-__global__ __launch_bounds__(W * 64) void w4_kernel(W4Args a) {
+// Where the lanes of a matrix instruction find their tokens in memory: the
+// caller's rows, or packed ones. Elements.
+struct Tokens {
+  const void* x;
+  int64_t row;       // from a lane's row to the next (packed: from lane to lane)
+  int64_t tile;      // from a tile of 16 tokens to the next
+  int64_t chunk;     // from a workgroup's tiles to the next one's
+  int step, block;   // from 32 columns to the next, from 128 to the next
+  int columns, packed;
+};
+
+// What is read for columns past the last.
+__device__ const u32x4 kNothing = {0, 0, 0, 0};
+
+// MT tiles of 16 tokens, NT tiles of 16 weight rows, groups of G columns. kX:
+// tokens come through LDS, else from memory.
+template <typename T, int MT, int NT, int G, bool kZeros, bool kX, int W>
+__global__ __launch_bounds__(W * 64) void w4_kernel(W4Args a, Tokens from) {
   using x8 = typename Mat<T>::x8;
-  constexpr int kSubs = 128 / G;      // groups of a block of 128 columns
-  constexpr int kSteps = G / 32;      // matrix instructions of a group
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  constexpr int kSubs = 128 / G;  // groups of a block of 128 columns
+  constexpr int kSteps = G / 32;  // matrix instructions of a group
+  extern __shared__ u32x4 lds[];
+  const Lds<T, MT, NT> plan(a, kX, W);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 15, g = lane >> 4;
   const int tiles = (a.n + 15) >> 4, blocks = (a.k + 127) >> 7;
-  const int groups = (a.k + G - 1) / G;
+  const int groups = plan.groups;
   const int tile0 = blockIdx.x * NT, m0 = blockIdx.y * 16 * MT;
 
-  const T* x[MT];
-  bool live[MT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int m = m0 + mt * 16 + r;
-    live[mt] = m < a.m;
-    x[mt] = (const T*)a.x + (int64_t)(live[mt] ? m : 0) * a.ldx;
-  }
   const u32x4* codes[NT];
-  const T* scales[NT];
-  const uint8_t* zeros[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int tile = tile0 + nt < tiles ? tile0 + nt : tiles - 1;
     codes[nt] = (const u32x4*)a.codes + (int64_t)tile * blocks * 64 + lane;
-    scales[nt] = (const T*)a.scales + (int64_t)tile * groups * 16 + g * 4;
-    zeros[nt] = kZeros ? a.zeros + (int64_t)tile * groups * 16 + r : nullptr;
+  }
+  const T* x[MT];
+  if constexpr (!kX) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {  // tokens past the last are another's: their results go nowhere
+      const int m = mt * 16 + r, last = a.m - m0 - 1;
+      x[mt] = (const T*)from.x + blockIdx.y * from.chunk;
+      x[mt] += from.packed ? mt * from.tile + lane * 8 : (m < last ? m : last) * from.row + g * 8;
+    }
+  }
+  // The next turn's codes come from memory while this one's are at work, and
+  // its tokens, kRing steps ahead, into the registers that a step leaves.
+  constexpr int kRing = kX || MT <= 2 ? 4 : 2;
+  constexpr bool kLate = kSteps > kRing;  // a group's tokens are never all here
+  u32x4 now[NT], next[NT];
+  x8 xf[MT][kRing];
+  auto load_codes = [&](int b) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) next[nt] = __builtin_nontemporal_load(codes[nt] + (int64_t)b * 64);
+  };
+  auto load_x = [&](int b, int j) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const T* p = x[mt] + (int64_t)b * from.block + j * from.step;
+      if constexpr (MT == 1)  // more are packed, with zeros behind the last column
+        p = b * 128 + j * 32 + g * 8 < from.columns ? p : (const T*)&kNothing;
+      xf[mt][j % kRing] = *reinterpret_cast<const x8*>(p);
+    }
+  };
+  if (wave < blocks) {
+    load_codes(wave);
+    if constexpr (!kX) {
+#pragma unroll
+      for (int j = 0; j < kRing; ++j) load_x(wave, j);
+    }
+  }
+
+  // scales, zero points and few tokens are small pieces scattered over lanes:
+  // read from memory each would cost a load as long as one of codes
+  char* base = reinterpret_cast<char*>(lds);
+  T* scales = reinterpret_cast<T*>(base);
+  uint8_t* zeros = reinterpret_cast<uint8_t*>(base + plan.scales);
+  T* xs = reinterpret_cast<T*>(base + plan.scales + plan.zeros);
+  {
+    const int rest = (tiles - tile0 < NT ? tiles - tile0 : NT) * groups * 16;  // of the tiles that are there
+    const T* sc = (const T*)a.scales + (int64_t)tile0 * groups * 16;
+    for (int i = threadIdx.x * 4; i < rest; i += W * 256)
+      *reinterpret_cast<u32x2*>(scales + i) = *reinterpret_cast<const u32x2*>(sc + i);
+    if constexpr (kZeros) {
+      const uint8_t* z = a.zeros + (int64_t)tile0 * groups * 16;
+      for (int i = threadIdx.x * 4; i < rest; i += W * 256)
+        *reinterpret_cast<uint32_t*>(zeros + i) = *reinterpret_cast<const uint32_t*>(z + i);
+    }
+    if constexpr (kX) {
+      const int rows = a.m - m0 < 16 * MT ? a.m - m0 : 16 * MT;
+      const bool whole = a.k % 8 == 0 && a.ldx % 8 == 0 && (uintptr_t)a.x % 16 == 0;
+      for (int row = 0; row < rows; ++row) {
+        const T* src = (const T*)a.x + (int64_t)(m0 + row) * a.ldx;
+        for (int k = threadIdx.x * 8; k < blocks * 128; k += W * 512) {
+          x8 v = bits_as<x8>(u32x4{0, 0, 0, 0});
+          if (whole) {
+            if (k < a.k) v = *reinterpret_cast<const x8*>(src + k);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (k + i < a.k) v[i] = src[k + i];
+          }
+          *reinterpret_cast<x8*>(xs + row * plan.pitch + k) = v;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  int at[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int last = a.m - m0 - 1;
+    at[mt] = (mt * 16 + r < last ? mt * 16 + r : last) * plan.pitch + g * 8;
   }
 
   f32x4 acc[NT][MT] = {};
-  const x8 eight = splat8<T>(-24.f);  // -(16 + 8)
+  const Decoder<T> decode;
+  const x8 offset = splat8<T>(kZeros ? -16.f : -24.f);  // 24: 16 + 8
+#pragma unroll 1
   for (int b = wave; b < blocks; b += W) {
-    u32x4 c[NT];
+    const int after = b + W < blocks ? b + W : b;  // the last turn reads its own again
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) c[nt] = codes[nt][(int64_t)b * 64];
-    x8 xf[MT][4];
+    for (int nt = 0; nt < NT; ++nt) now[nt] = next[nt];
+    if constexpr (kX) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        xf[mt][j] = load_x8<T, kVec>(x[mt], b * 128 + j * 32 + g * 8, a.k, live[mt]);
+        for (int j = 0; j < 4; ++j) xf[mt][j] = *reinterpret_cast<const x8*>(xs + at[mt] + b * 128 + j * 32);
+    }
+    load_codes(after);
 #pragma unroll
     for (int s = 0; s < kSubs; ++s) {
       int grp = b * kSubs + s;
       if (grp >= groups) grp = groups - 1;  // columns past the last: x is 0
-      f32x4 part[NT][MT];
-      if constexpr (!kZeros) {
+      f32x4 z[MT] = {}, part[NT][MT];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          f32x4 z = {};
+      for (int mt = 0; mt < MT; ++mt) {
+        if constexpr (!kLate) {
 #pragma unroll
-          for (int j = 0; j < kSteps; ++j) z = Mat<T>::mfma(eight, xf[mt][s * kSteps + j], z);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) part[nt][mt] = z;
+          for (int j = 0; j < kSteps; ++j) z[mt] = Mat<T>::mfma(offset, xf[mt][(s * kSteps + j) % kRing], z[mt]);
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) part[nt][mt] = z[mt];
+      }
+#pragma unroll
+      for (int j = s * kSteps; j < (s + 1) * kSteps; ++j) {
+        if constexpr (kLate) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) z[mt] = Mat<T>::mfma(offset, xf[mt][j % kRing], z[mt]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const x8 w = decode(now[nt][j]);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) part[nt][mt] = Mat<T>::mfma(w, xf[mt][j % kRing], part[nt][mt]);
+        }
+        if constexpr (!kX) load_x(j + kRing < 4 ? b : after, (j + kRing) % 4);
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        if constexpr (kZeros) {
-          const x8 off = splat8<T>(-16.f - (float)zeros[nt][grp * 16]);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            f32x4 z = {};
-#pragma unroll
-            for (int j = 0; j < kSteps; ++j) z = Mat<T>::mfma(off, xf[mt][s * kSteps + j], z);
-            part[nt][mt] = z;
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-          const x8 w = decode8<T>(c[nt][s * kSteps + j]);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-            part[nt][mt] = Mat<T>::mfma(w, xf[mt][s * kSteps + j], part[nt][mt]);
-        }
-        const u32x2 raw = *reinterpret_cast<const u32x2*>(scales[nt] + grp * 16);
-        typedef T t4 __attribute__((ext_vector_type(4)));
-        const t4 sc = bits_as<t4>(raw);
+        const int place = (nt * groups + grp) * 16 + g * 4;
+        const t4 sc = bits_as<t4>(*reinterpret_cast<const u32x2*>(scales + place));
+        uint32_t zp = 0;
+        if constexpr (kZeros) zp = *reinterpret_cast<const uint32_t*>(zeros + place);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[nt][mt][i] += (float)sc[i] * part[nt][mt][i];
+          for (int i = 0; i < 4; ++i) {
+            float v = kLate ? part[nt][mt][i] + z[mt][i] : part[nt][mt][i];
+            if constexpr (kZeros)  // z is -16 times the sum of x
+              v = __builtin_fmaf((float)(zp >> (8 * i) & 255u), z[mt][i] * 0.0625f, v);
+            acc[nt][mt][i] = __builtin_fmaf((float)sc[i], v, acc[nt][mt][i]);
+          }
       }
+      if constexpr (MT * NT > 4) __builtin_amdgcn_sched_barrier(0);  // registers
     }
   }
 
-  __shared__ f32x4 sums[W][NT * MT][64];
+  __syncthreads();  // what was staged has been used
+  f32x4* sums = reinterpret_cast<f32x4*>(lds);  // [W][NT MT][64]
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) sums[wave][nt * MT + mt][lane] = acc[nt][mt];
+    for (int mt = 0; mt < MT; ++mt) sums[(wave * NT * MT + nt * MT + mt) * 64 + lane] = acc[nt][mt];
   __syncthreads();
   for (int f = wave; f < NT * MT; f += W) {
-    f32x4 s = sums[0][f][lane];
+    f32x4 s = sums[f * 64 + lane];
 #pragma unroll
-    for (int w = 1; w < W; ++w) s += sums[w][f][lane];
+    for (int w = 1; w < W; ++w) s += sums[(w * NT * MT + f) * 64 + lane];
     const int m = m0 + (f % MT) * 16 + r;
     const int n = (tile0 + f / MT) * 16 + g * 4;
     if (m < a.m) {
@@ -178,41 +290,100 @@ __global__ __launch_bounds__(W * 64) void w4_kernel(W4Args a) {
   }
 }
 
-template <typename T, int MT, int NT, int G, bool kZeros, bool kVec>
+// Tokens in the order of the matrix instruction's loads, 1 KB for 16 tokens and
+// 32 columns; columns and tokens past the last are 0. A wave each.
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(W4Args a, T* to, int mts, bool whole) {
+  typedef typename Mat<T>::x8 x8;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int pieces = (a.k + 127) / 128 * 4 * mts;  // of a chunk of mts tiles
+  const int piece = blockIdx.x * 4 + wave;
+  if (piece >= pieces) return;
+  const int m = (blockIdx.y * mts + piece % mts) * 16 + (lane & 15);
+  const int k = piece / mts * 32 + (lane >> 4) * 8;
+  x8 v = bits_as<x8>(u32x4{0, 0, 0, 0});
+  if (m < a.m) {
+    const T* src = (const T*)a.x + m * a.ldx + k;
+    if (whole) {
+      if (k < a.k) v = *reinterpret_cast<const x8*>(src);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k + i < a.k) v[i] = src[i];
+    }
+  }
+  *reinterpret_cast<x8*>(to + ((int64_t)blockIdx.y * pieces + piece) * 512 + lane * 8) = v;
+}
+
+constexpr int kWaves = 8;
+
+int token_tiles(int m) { return m <= 16 ? 1 : m <= 32 ? 2 : 4; }
+bool whole_loads(const W4Args& a) { return a.k % 8 == 0 && a.ldx % 8 == 0 && (uintptr_t)a.x % 16 == 0; }
+bool through_lds(const W4Args& a) { return a.m <= 16 && (int64_t)a.m * a.k <= 16384; }
+bool packs(const W4Args& a) {
+  return !through_lds(a) && (a.m > 16 || !whole_loads(a));
+}
+
+template <typename T, int MT, int NT, int G, bool kZeros, bool kX>
 hipError_t launch(const W4Args& a, hipStream_t stream) {
-  constexpr int W = 8;
-  const int tiles = (a.n + 15) / 16;
-  const dim3 grid((tiles + NT - 1) / NT, (a.m + 16 * MT - 1) / (16 * MT));
-  w4_kernel<T, MT, NT, G, kZeros, kVec, W><<<grid, W * 64, 0, stream>>>(a);
+  const int tiles = (a.n + 15) / 16, blocks = (a.k + 127) / 128;
+  const int chunks = (a.m + 16 * MT - 1) / (16 * MT);
+  Tokens from{a.x, a.ldx, 0, 16 * MT * a.ldx, 32, 128, a.k, 0};
+  if (!kX && packs(a)) {
+    const int pieces = blocks * 4 * MT;
+    pack_kernel<T><<<dim3((pieces + 3) / 4, chunks), 256, 0, stream>>>(a, (T*)a.work, MT, whole_loads(a));
+    if (hipError_t e = hipGetLastError()) return e;
+    from = Tokens{a.work, 8, 512, (int64_t)pieces * 512, MT * 512, MT * 2048, blocks * 128, 1};
+  }
+  const Lds<T, MT, NT> plan(a, kX, kWaves);
+  auto kernel = w4_kernel<T, MT, NT, G, kZeros, kX, kWaves>;
+  if (plan.size > 65536) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)plan.size);
+    if (e != hipSuccess) return e;
+  }
+  kernel<<<dim3((tiles + NT - 1) / NT, chunks), kWaves * 64, plan.size, stream>>>(a, from);
   return hipGetLastError();
 }
 
-template <typename T, int MT, int NT, int G, bool kZeros>
-hipError_t by_load(const W4Args& a, hipStream_t stream) {
-  const bool vec = a.k % 8 == 0 && a.ldx % 8 == 0 && (uintptr_t)a.x % 16 == 0;
-  return vec ? launch<T, MT, NT, G, kZeros, true>(a, stream) : launch<T, MT, NT, G, kZeros, false>(a, stream);
-}
-
-template <typename T, int MT, int NT>
+template <typename T, int MT, int NT, bool kX>
 hipError_t by_group(const W4Args& a, hipStream_t stream) {
   if (a.zeros) {
-    if (a.group == 32) return by_load<T, MT, NT, 32, true>(a, stream);
-    if (a.group == 64) return by_load<T, MT, NT, 64, true>(a, stream);
-    return by_load<T, MT, NT, 128, true>(a, stream);
+    if (a.group == 32) return launch<T, MT, NT, 32, true, kX>(a, stream);
+    if (a.group == 64) return launch<T, MT, NT, 64, true, kX>(a, stream);
+    return launch<T, MT, NT, 128, true, kX>(a, stream);
   }
-  if (a.group == 32) return by_load<T, MT, NT, 32, false>(a, stream);
-  if (a.group == 64) return by_load<T, MT, NT, 64, false>(a, stream);
-  return by_load<T, MT, NT, 128, false>(a, stream);
+  if (a.group == 32) return launch<T, MT, NT, 32, false, kX>(a, stream);
+  if (a.group == 64) return launch<T, MT, NT, 64, false, kX>(a, stream);
+  return launch<T, MT, NT, 128, false, kX>(a, stream);
+}
+
+template <typename T, int MT>
+hipError_t by_rows(const W4Args& a, hipStream_t stream) {
+  const int tiles = (a.n + 15) / 16;
+  // scales of more tiles than one have to leave room in the LDS
+  auto fits = [&](int nt) { return nt * ((a.k + a.group - 1) / a.group) * 48 <= 98304; };
+  if (tiles >= 1024 && fits(4)) return by_group<T, MT, 4, false>(a, stream);
+  if (tiles >= 512 && fits(2)) return by_group<T, MT, 2, false>(a, stream);
+  return by_group<T, MT, 1, false>(a, stream);
 }
 
 template <typename T>
 hipError_t by_tokens(const W4Args& a, hipStream_t stream) {
-  if (a.m <= 16) return by_group<T, 1, 1>(a, stream);
-  if (a.m <= 32) return by_group<T, 2, 1>(a, stream);
-  return by_group<T, 4, 1>(a, stream);
+  if (through_lds(a)) return by_group<T, 1, 1, true>(a, stream);
+  switch (token_tiles(a.m)) {
+    case 1: return by_rows<T, 1>(a, stream);
+    case 2: return by_rows<T, 2>(a, stream);
+    default: return by_rows<T, 4>(a, stream);
+  }
 }
 
 }  // namespace
+
+int64_t w4_workspace(const W4Args& a) {
+  if (!packs(a)) return 0;
+  const int mts = token_tiles(a.m);
+  return (int64_t)((a.m + 16 * mts - 1) / (16 * mts)) * ((a.k + 127) / 128) * 4 * mts * 1024;
+}
 
 hipError_t launch_w4_matmul(const W4Args& a, hipStream_t stream) {
   return a.dtype == kBF16 ? by_tokens<__bf16>(a, stream) : by_tokens<_Float16>(a, stream);

@@ -48,6 +48,7 @@ _CODES = (torch.float8_e4m3fn, torch.uint8)
 _INT_MAX = 2**31 - 1
 
 GROUPS = (32, 64, 128)
+MAX_COLUMNS = _serving.MAX_COLUMNS
 MAX_TOP = _serving.MAX_TOP
 MAX_VOCAB = _serving.MAX_VOCAB
 MAX_HEAD_DIM = 256
@@ -159,8 +160,8 @@ def w4_matmul(
     ``x`` is [M, K] in bf16 or fp16, its rows at any stride; ``codes``,
     ``scales`` (x's type) and ``zeros`` are as :func:`pack_w4` lays them out
     (no zeros: every zero point is 8). Meant for the tokens of a decode batch,
-    M up to 64; larger M are taken 64 rows at a time. Sums are fp32, rounded
-    once to x's type. ``x`` has to be finite, and under 1e37 in magnitude.
+    M up to 64; larger M are taken 64 rows at a time, K up to ``MAX_COLUMNS``.
+    Sums are fp32, rounded once to x's type. ``x`` has to be finite, and under 1e37 in magnitude.
     """
     _check_input("x", x, None, (torch.bfloat16, torch.float16), 2)
     device = x.device
@@ -168,7 +169,7 @@ def w4_matmul(
     n = int(out_features)
     if group_size not in GROUPS:
         raise ValueError(f"group_size must be one of {GROUPS}, not {group_size}")
-    if k < 1 or n < 1 or k > _INT_MAX // 2 or n > _INT_MAX // 2 or m > 65535 * 16:
+    if k < 1 or n < 1 or k > MAX_COLUMNS or n > _INT_MAX // 2 or m > 65535 * 16:
         raise ValueError(f"no product of {m} rows with weights [{n}, {k}]")
     tiles, groups = -(-n // 16), -(-k // group_size)
     _check_input("codes", codes, device, (torch.uint8,), 4)
@@ -193,9 +194,12 @@ def w4_matmul(
     if x.stride(1) != 1 and k > 1:
         x = x.contiguous()
     if m:
+        args = (x.data_ptr(), x.stride(0), m, n, k, group_size, _DTYPES[x.dtype])
+        size = _serving.w4_workspace(*args)
+        work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         _serving.w4_matmul(
-            device.index, _stream(device), x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(),
-            0 if zeros is None else zeros.data_ptr(), out.data_ptr(), out.stride(0), m, n, k, group_size, _DTYPES[x.dtype],
+            device.index, _stream(device), *args, codes.data_ptr(), scales.data_ptr(),
+            0 if zeros is None else zeros.data_ptr(), out.data_ptr(), out.stride(0), work.data_ptr() if size else 0,
         )
     return out
 

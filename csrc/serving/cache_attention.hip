@@ -23,6 +23,8 @@
 // A workgroup's 4 waves take turns at tiles of 64 tokens and join in LDS. Long
 // contexts are split over workgroups in chunks of a fixed number of tokens,
 // whose results a second launch joins in their order.
+#include <type_traits>
+
 #include "device.h"
 #include "geometry.h"
 #include "serving.h"
@@ -74,8 +76,10 @@ __device__ __forceinline__ void store4(T* to, f32x4 v) {
 }
 
 // DT tiles of 16 dimensions, QT tiles of 16 query rows.
+constexpr int waves_of(int dt, int qt) { return dt * qt <= 4 ? 3 : dt * qt <= 8 ? 2 : 1; }
+
 template <typename T, int DT, int QT>
-__global__ __launch_bounds__(kWaves * 64) void attention_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kernel(AttentionArgs a) {
   using x8 = typename Mat<T>::x8;
   constexpr int KB = DT / 4;  // blocks of 64 dimensions
   const CacheArgs& c = a.c;
@@ -96,12 +100,13 @@ __global__ __launch_bounds__(kWaves * 64) void attention_kernel(AttentionArgs a)
 
   // the lane's query rows, their positions, and their operands
   x8 q[QT][KB * 2];
-  int pos[QT];
+  int pos[QT], low[QT];  // a row sees the positions low + 1 .. pos
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int i = t * 16 + r < p.rows ? t * 16 + r : p.rows - 1;
     const int tok = (p.local + i) / group, head = h * group + (p.local + i) % group;
     pos[t] = p.len - p.count + tok;
+    low[t] = a.window ? pos[t] - a.window : -1;
     const T* src = (const T*)a.q + (int64_t)(p.row0 + tok) * a.q_row + head * a.q_head;
 #pragma unroll
     for (int k = 0; k < KB * 2; ++k) {
@@ -111,141 +116,189 @@ __global__ __launch_bounds__(kWaves * 64) void attention_kernel(AttentionArgs a)
     }
   }
 
-  f32x4 acc[QT][DT] = {};
+  f32x4 acc[QT][DT];
   float top[QT], sum[QT];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    top[t] = -kInf;
-    sum[t] = 0.f;
-  }
-  const float unit = a.scale * kLog2e;
-
-  for (int base = begin + wave * kTile; base < end; base += kWaves * kTile) {
-    const int tok0 = base + g * 16;  // the lane's 16 tokens for P and V
-    // pages by groups of 16 tokens; one that is out of range gives NaN
-    const int blk = tok0 >> shift;
-    int pid = blk < c.blocks && tok0 < end ? table[blk] : -1;
-    const bool known = pid >= 0 && pid < c.pages && !p.broken;
-    if (pid < 0 || pid >= c.pages) pid = 0;
-    const int pid_k = __shfl(pid, (r >> 2) << 4);
-    const int64_t ph = (int64_t)pid * c.heads + h, ph_k = (int64_t)pid_k * c.heads + h;
-    const uint8_t* kp = c.k + (ph_k * page + ((base + ((r >> 2) << 4)) & (page - 1)) + (r & 3)) * dim + g * 16;
-    const uint8_t* vp = c.v + (ph * dim + r) * page + (tok0 & (page - 1));
-
-    u32x4 kr[4][KB], vr[DT];
+  // Keys of the next tile come while this one's weights are formed, and this
+  // tile's values while its scores are: each takes the registers that the other
+  // has left. Page numbers come a tile ahead of the keys.
+  struct Pages {
+    int pid;     // of the lane's 16 tokens, within range
+    bool known;  // whether it was; if not, what sees it is NaN
+  };
+  auto look_up = [&](int base) {
+    const int blk = (base + g * 16) >> shift;
+    const int pid = table[blk < c.blocks ? blk : c.blocks - 1];
+    const bool known = blk < c.blocks && (uint32_t)pid < (uint32_t)c.pages && !p.broken;
+    return Pages{(uint32_t)pid < (uint32_t)c.pages ? pid : 0, known};
+  };
+  u32x4 kr[4][KB], vr[DT];
+  float ks, vs;
+  auto load_keys = [&](int base, const Pages& at) {
+    const int pid = __shfl(at.pid, (r >> 2) << 4);
+    const int tok = ((base + ((r >> 2) << 4)) & (page - 1)) + (r & 3);
+    const uint8_t* from = c.k + (((int64_t)pid * c.heads + h) * page + tok) * dim + g * 16;
 #pragma unroll
     for (int m = 0; m < 4; ++m)
 #pragma unroll
       for (int k = 0; k < KB; ++k) {
-        kr[m][k] = u32x4{0, 0, 0, 0};
-        if (k * 64 + g * 16 < dim) kr[m][k] = *reinterpret_cast<const u32x4*>(kp + m * 4 * dim + k * 64);
+        const uint8_t* here = from + m * 4 * dim + k * 64;
+        if (k * 64 + g * 16 >= dim) here = from - g * 16;  // the queries are 0 there
+        kr[m][k] = *reinterpret_cast<const u32x4*>(here);
       }
-    float ks = known ? c.k_scale[ph] * unit : __builtin_nanf("");
-    float vs = known ? c.v_scale[ph] : 1.f;
+    const int64_t ph = (int64_t)at.pid * c.heads + h;
+    ks = c.k_scale[ph];
+    vs = c.v_scale[ph];
+  };
+  auto load_values = [&](int base, const Pages& at) {
+    const uint8_t* from = c.v + (((int64_t)at.pid * c.heads + h) * dim + r) * page + ((base + g * 16) & (page - 1));
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      vr[d] = u32x4{0, 0, 0, 0};
-      if (d * 16 < dim) vr[d] = *reinterpret_cast<const u32x4*>(vp + (int64_t)d * 16 * page);
-    }
-    if (tok0 >= end) vs = 1.f;
-    const float vlog = __builtin_amdgcn_logf(vs);
+    for (int d = 0; d < DT; ++d)
+      vr[d] = *reinterpret_cast<const u32x4*>(from + (d * 16 < dim ? d : 0) * 16 * page);
+  };
 
-    const bool edge = base + kTile > p.first + 1 || (a.window && base <= p.last - a.window);
-    bool odd = false;
-    if (edge) {
-      // values that no row sees are whatever the page held before
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          vr[d][w] &= bytes_below(p.hi - tok0 - 4 * w) & ~bytes_below(p.lo - tok0 - 4 * w);
-          odd |= nan_bytes(vr[d][w]) != 0;
-        }
-      odd = __any(odd);
-    }
-
-    f16x8 pw[QT][2];
-    f16x8 seen[QT][2];
+  // Takes the wave's tiles. A tile at the edge of what the rows see may hold
+  // NaN among the values of some of them: then `sweep` says so, and the second
+  // form, which keeps a NaN from the rows that do not see it, starts over.
+  auto sweep = [&](auto careful) {
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      f32x4 s[4] = {};
+      top[t] = -kInf;
+      sum[t] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    int base = begin + wave * kTile;
+    if (base >= end) return false;
+    bool odd = false;
+    Pages here = look_up(base);
+    load_keys(base, here);
+    Pages next = look_up(base + kWaves * kTile < end ? base + kWaves * kTile : base);
+#pragma unroll 1
+    for (; base < end; base += kWaves * kTile) {
+      const int tok0 = base + g * 16;  // the lane's 16 tokens for P and V
+      load_values(base, here);
+      const float unit = here.known ? ks * a.scale * kLog2e : __builtin_nanf("");
+      const float weight = here.known && tok0 < end ? vs : 1.f;
+      const float vlog = __builtin_amdgcn_logf(weight);
+
+      f32x4 s[QT][4] = {};
 #pragma unroll
       for (int m = 0; m < 4; ++m)
 #pragma unroll
         for (int k = 0; k < KB; ++k) {
-          s[m] = Mat<T>::mfma(Codes<T>::widen(kr[m][k][0], kr[m][k][1]), q[t][2 * k], s[m]);
-          s[m] = Mat<T>::mfma(Codes<T>::widen(kr[m][k][2], kr[m][k][3]), q[t][2 * k + 1], s[m]);
-        }
-      float best = -kInf;
+          const x8 lo = Codes<T>::widen(kr[m][k][0], kr[m][k][1]), hi = Codes<T>::widen(kr[m][k][2], kr[m][k][3]);
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[m][i] *= ks;
-          if (edge) {
-            const int j = tok0 + m * 4 + i;
-            const bool in = j <= pos[t] && (!a.window || j > pos[t] - a.window);
-            if (!in) s[m][i] = -kInf;
-            seen[t][m >> 1][(m & 1) * 4 + i] = in ? (_Float16)1.f : (_Float16)0.f;
+          for (int t = 0; t < QT; ++t) {
+            s[t][m] = Mat<T>::mfma(lo, q[t][2 * k], s[t][m]);
+            s[t][m] = Mat<T>::mfma(hi, q[t][2 * k + 1], s[t][m]);
           }
-          best = fmaxf(best, s[m][i]);
         }
-      best += vlog;
-      best = fmaxf(best, __shfl_xor(best, 16));
-      best = fmaxf(best, __shfl_xor(best, 32));
-      const float now = fmaxf(top[t], best);
-      const float ref = now == -kInf ? 0.f : now;
-      if (__any(now != top[t])) {
-        const float f = __builtin_amdgcn_exp2f(top[t] - ref);
-        sum[t] *= f;
+      const int ahead = base + kWaves * kTile < end ? base + kWaves * kTile : base;  // the last reads its own again
+      load_keys(ahead, next);
+      here = next;
+      next = look_up(ahead + kWaves * kTile < end ? ahead + kWaves * kTile : ahead);
+
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[t][d] *= f;
-      }
-      top[t] = now;
+      for (int t = 0; t < QT; ++t)
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(s[m][i] - ref);
-          sum[t] += e;
-          pw[t][m >> 1][(m & 1) * 4 + i] = (_Float16)(e * vs);
-        }
-    }
-    if (odd) {
-      // a NaN among the values reaches the rows that see it, and no others
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        f32x4 hits[QT] = {};
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          uint32_t w0 = nan_bytes(vr[d][2 * x]) >> 7, w1 = nan_bytes(vr[d][2 * x + 1]) >> 7;
-          vr[d][2 * x] &= ~(w0 * 0xFFu);
-          vr[d][2 * x + 1] &= ~(w1 * 0xFFu);
-          f16x8 is;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            is[i] = (_Float16)(float)(w0 >> (8 * i) & 1u);
-            is[4 + i] = (_Float16)(float)(w1 >> (8 * i) & 1u);
-          }
-#pragma unroll
-          for (int t = 0; t < QT; ++t) hits[t] = Mat<_Float16>::mfma(is, seen[t][x], hits[t]);
-        }
+        for (int m = 0; m < 4; ++m) s[t][m] *= unit;
+      const bool edge = base + kTile > p.first + 1 || (a.window && base <= p.last - a.window);
+      if (edge) {
 #pragma unroll
         for (int t = 0; t < QT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (hits[t][i] > 0.f) acc[t][d][i] = __builtin_nanf("");
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int j = tok0 + m * 4 + i;
+              const bool in = (j <= pos[t]) & (j > low[t]);
+              s[t][m][i] = in ? s[t][m][i] : -kInf;
+            }
       }
+      f16x8 pw[QT][2];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        float best = -kInf;
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) best = fmaxf(best, s[t][m][i]);
+        best += vlog;
+        best = fmaxf(best, __shfl_xor(best, 16));
+        best = fmaxf(best, __shfl_xor(best, 32));
+        const float now = fmaxf(top[t], best);
+        const float ref = now == -kInf ? 0.f : now;
+        if (__any(now != top[t])) {
+          const float f = __builtin_amdgcn_exp2f(top[t] - ref);
+          sum[t] *= f;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) acc[t][d] *= f;
+        }
+        top[t] = now;
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = __builtin_amdgcn_exp2f(s[t][m][i] - ref);
+            sum[t] += e;
+            pw[t][m >> 1][(m & 1) * 4 + i] = (_Float16)(e * weight);
+          }
+      }
+      if (edge) {
+        // values that no row sees are whatever the page held before
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t keep = bytes_below(p.hi - tok0 - 4 * w) & ~bytes_below(p.lo - tok0 - 4 * w);
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            vr[d][w] &= keep;
+            odd |= nan_bytes(vr[d][w]) != 0;
+          }
+        }
+        if constexpr (careful) {
+          f16x8 seen[QT][2];
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              seen[t][i >> 3][i & 7] = (tok0 + i <= pos[t]) & (tok0 + i > low[t]) ? (_Float16)1.f : (_Float16)0.f;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            f32x4 hits[QT] = {};
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const uint32_t w0 = nan_bytes(vr[d][2 * x]) >> 7, w1 = nan_bytes(vr[d][2 * x + 1]) >> 7;
+              vr[d][2 * x] &= ~(w0 * 0xFFu);
+              vr[d][2 * x + 1] &= ~(w1 * 0xFFu);
+              f16x8 is;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                is[i] = (_Float16)(float)(w0 >> (8 * i) & 1u);
+                is[4 + i] = (_Float16)(float)(w1 >> (8 * i) & 1u);
+              }
+#pragma unroll
+              for (int t = 0; t < QT; ++t) hits[t] = Mat<_Float16>::mfma(is, seen[t][x], hits[t]);
+            }
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (hits[t][i] > 0.f) acc[t][d][i] = __builtin_nanf("");
+          }
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const f16x8 v = Codes<_Float16>::widen(vr[d][2 * x], vr[d][2 * x + 1]);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) acc[t][d] = Mat<_Float16>::mfma(v, pw[t][x], acc[t][d]);
+        }
     }
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const f16x8 v = Codes<_Float16>::widen(vr[d][2 * x], vr[d][2 * x + 1]);
-#pragma unroll
-        for (int t = 0; t < QT; ++t) acc[t][d] = Mat<_Float16>::mfma(v, pw[t][x], acc[t][d]);
-      }
-  }
+    return __any(odd) != 0;
+  };
+  if (sweep(std::false_type{})) sweep(std::true_type{});
 
   // the waves' parts: against one reference, then summed in the waves' order
   __shared__ float tops[kWaves][QT][16], sums[kWaves][QT][16];

@@ -24,16 +24,19 @@ struct Place {
   bool broken;              // longer than its row of the table: its results are NaN
 };
 
+// Rows of a tile are a power of two.
+__host__ __device__ inline int tile_shift(const AttentionArgs& a) { return __builtin_ctz(a.row_tile); }
+
 // Slots of sequence b start at starts[b] group / row_tile + b: enough for its
 // tiles, whatever the lengths, and a rule that a binary search can invert.
 __host__ __device__ inline int64_t first_slot(const AttentionArgs& a, int group, int b) {
-  return (int64_t)a.c.starts[b] * group / a.row_tile + b;
+  return ((int64_t)a.c.starts[b] * group >> tile_shift(a)) + b;
 }
 
 __host__ __device__ inline int64_t slot_count(const AttentionArgs& a) {
   const int group = a.q_heads / a.c.heads;
-  if (!a.c.starts) return (int64_t)a.c.batch * ((group + a.row_tile - 1) / a.row_tile);
-  return (int64_t)a.c.rows * group / a.row_tile + a.c.batch + 1;
+  if (!a.c.starts) return (int64_t)a.c.batch * ((group + a.row_tile - 1 >> tile_shift(a)));
+  return ((int64_t)a.c.rows * group >> tile_shift(a)) + a.c.batch + 1;
 }
 
 // The rest of `p` from b, count and tile.
@@ -52,7 +55,7 @@ __host__ __device__ inline void fill_place(const AttentionArgs& a, int group, Pl
   p.hi = p.last + 1 > 0 ? p.last + 1 : 0;
   p.lo = a.window && p.first - a.window + 1 > 0 ? p.first - a.window + 1 : 0;
   const int start = p.lo & ~(kTile - 1);
-  const int n = p.hi > start ? (int)(((int64_t)p.hi - start + a.chunk - 1) / a.chunk) : 1;
+  const int n = p.hi > start ? (int)((uint32_t)(p.hi - start - 1) / (uint32_t)a.chunk) + 1 : 1;
   p.splits = n < a.splits ? n : a.splits;
 }
 
@@ -74,7 +77,7 @@ __host__ __device__ inline bool place_of_slot(const AttentionArgs& a, int group,
     if (tile < 0 || tile * a.row_tile >= (int64_t)p.count * group) return false;
     p.tile = (int)tile;
   } else {
-    const int per = (group + a.row_tile - 1) / a.row_tile;
+    const int per = (group + a.row_tile - 1 >> tile_shift(a));
     p.b = p.row0 = slot / per;
     p.tile = slot - p.b * per;
     p.count = 1;
@@ -104,10 +107,10 @@ __host__ __device__ inline bool place_of_row(const AttentionArgs& a, int group, 
   } else {
     p.b = p.row0 = row;
     p.count = 1;
-    slot = (int64_t)row * ((group + a.row_tile - 1) / a.row_tile);
+    slot = (int64_t)row * ((group + a.row_tile - 1 >> tile_shift(a)));
   }
   const int local = (row - p.row0) * group + head % group;
-  p.tile = local / a.row_tile;
+  p.tile = local >> tile_shift(a);
   index = local - p.tile * a.row_tile;
   slot += p.tile;
   fill_place(a, group, p);

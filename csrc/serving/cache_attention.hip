@@ -75,24 +75,38 @@ __device__ __forceinline__ void store4(T* to, f32x4 v) {
   *reinterpret_cast<t4*>(to) = r;
 }
 
-// DT tiles of 16 dimensions, QT tiles of 16 query rows.
+// DT tiles of 16 dimensions, all of them there if kWhole; QT tiles of 16 query
+// rows.
+// Codes that one workgroup reads once pass by the L2.
+template <int QT>
+__device__ __forceinline__ u32x4 load16(const uint8_t* p) {
+  if constexpr (QT == 1) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+  return *reinterpret_cast<const u32x4*>(p);
+}
+
 constexpr int waves_of(int dt, int qt) { return dt * qt <= 4 ? 3 : dt * qt <= 8 ? 2 : 1; }
 
-template <typename T, int DT, int QT>
+template <typename T, int DT, int QT, bool kWhole>
 __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kernel(AttentionArgs a) {
   using x8 = typename Mat<T>::x8;
   constexpr int KB = DT / 4;  // blocks of 64 dimensions
   const CacheArgs& c = a.c;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 15, g = lane >> 4;
-  const int h = blockIdx.y, split = blockIdx.z;
   const int group = a.q_heads / c.heads;
+  // Workgroups go to the 8 dies in turn. All heads of a slot and split follow
+  // one another on one die: their codes are neighbours in every page.
+  const int turn = blockIdx.x >> 3, h = turn % c.heads;
+  const int64_t job = (int64_t)(turn / c.heads) * 8 + (blockIdx.x & 7);
+  const int slots = (int)slot_count(a);
+  const int split = (int)(job / slots), slot = (int)(job - (int64_t)split * slots);
+  if (split >= a.splits) return;
 
   Place p;
-  if (!place_of_slot(a, group, blockIdx.x, p)) return;
+  if (!place_of_slot(a, group, slot, p)) return;
   if (split >= p.splits) return;
 
-  const int page = c.page, dim = c.dim;
+  const int page = c.page, dim = kWhole ? DT * 16 : c.dim;
   const int shift = 31 - __clz(page);
   const int begin = (p.lo & ~(kTile - 1)) + split * a.chunk;
   const int end = split == p.splits - 1 || begin + a.chunk > p.hi ? p.hi : begin + a.chunk;
@@ -112,7 +126,7 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
     for (int k = 0; k < KB * 2; ++k) {
       const int d = (k >> 1) * 64 + g * 16 + (k & 1) * 8;
       q[t][k] = bits_as<x8>(u32x4{0, 0, 0, 0});
-      if (d < dim) q[t][k] = *reinterpret_cast<const x8*>(src + d);
+      if (kWhole || d < dim) q[t][k] = *reinterpret_cast<const x8*>(src + d);
     }
   }
 
@@ -142,7 +156,7 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
 #pragma unroll
       for (int k = 0; k < KB; ++k) {
         const uint8_t* here = from + m * 4 * dim + k * 64;
-        if (k * 64 + g * 16 >= dim) here = from - g * 16;  // the queries are 0 there
+        if (!kWhole && k * 64 + g * 16 >= dim) here = from - g * 16;  // the queries are 0 there
         kr[m][k] = *reinterpret_cast<const u32x4*>(here);
       }
     const int64_t ph = (int64_t)at.pid * c.heads + h;
@@ -153,7 +167,7 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
     const uint8_t* from = c.v + (((int64_t)at.pid * c.heads + h) * dim + r) * page + ((base + g * 16) & (page - 1));
 #pragma unroll
     for (int d = 0; d < DT; ++d)
-      vr[d] = *reinterpret_cast<const u32x4*>(from + (d * 16 < dim ? d : 0) * 16 * page);
+      vr[d] = load16<QT>(from + (kWhole || d * 16 < dim ? d : 0) * 16 * page);
   };
 
   // Takes the wave's tiles. A tile at the edge of what the rows see may hold
@@ -339,19 +353,19 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
           f32x4 o = part[0][d][lane];
 #pragma unroll
           for (int w = 1; w < kWaves; ++w) o += part[w][d][lane];
-          if (d * 16 < dim) store4(out + d * 16, o * inv);
+          if (kWhole || d * 16 < dim) store4(out + d * 16, o * inv);
         }
         if (wave == 0 && g == 0)
           a.lse[(int64_t)(p.row0 + tok) * a.q_heads + head] = (all + __builtin_amdgcn_logf(total)) * kLn2;
       } else {
-        float* to = a.work + (((int64_t)blockIdx.x * c.heads + h) * a.splits + split) * a.row_tile * (dim + 2);
+        float* to = a.work + (((int64_t)slot * c.heads + h) * a.splits + split) * a.row_tile * (dim + 2);
         float* row = to + (int64_t)i * dim + g * 4;
 #pragma unroll
         for (int d = wave; d < DT; d += kWaves) {
           f32x4 o = part[0][d][lane];
 #pragma unroll
           for (int w = 1; w < kWaves; ++w) o += part[w][d][lane];
-          if (d * 16 < dim) *reinterpret_cast<f32x4*>(row + d * 16) = o;
+          if (kWhole || d * 16 < dim) *reinterpret_cast<f32x4*>(row + d * 16) = o;
         }
         if (wave == 0 && g == 0) {
           to[(int64_t)a.row_tile * dim + 2 * i] = all;
@@ -362,7 +376,8 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
   }
 }
 
-// Joins the splits of a row: one wave a row, four dimensions a lane.
+// Joins the splits of a row: one wave a row, four dimensions a lane. Lane s has
+// split s's reference and sum (a pass for each 64 splits).
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
   const CacheArgs& c = a.c;
@@ -380,26 +395,41 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
   const float* from = a.work + (slot * c.heads + h) * a.splits * a.row_tile * (dim + 2);
   const int64_t step = (int64_t)a.row_tile * (dim + 2);
   const float* heads = from + (int64_t)a.row_tile * dim + 2 * i;
-  float all = -kInf;
-  for (int s = 0; s < p.splits; ++s) all = fmaxf(all, heads[s * step]);
-  const float ref = all == -kInf ? 0.f : all;
-  float total = 0.f;
+  const int d = lane * 4 < dim ? lane * 4 : 0;
+  const float* mine = from + (int64_t)i * dim + d;
+  float all = -kInf, total = 0.f;
   f32x4 o = {};
-  const int d = lane * 4;
-  for (int s = 0; s < p.splits; ++s) {
-    const float f = __builtin_amdgcn_exp2f(heads[s * step] - ref);
-    total += heads[s * step + 1] * f;
-    if (d < dim) o += *reinterpret_cast<const f32x4*>(from + s * step + (int64_t)i * dim + d) * f;
+  for (int first = 0; first < p.splits; first += 64) {
+    const int n = p.splits - first < 64 ? p.splits - first : 64;
+    const float* at64 = heads + (first + (lane < n ? lane : 0)) * step;
+    const float top = at64[0], sum = at64[1];
+    const bool live = lane < n;
+    float best = live ? top : -kInf;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) best = fmaxf(best, __shfl_xor(best, x));
+    const float now = fmaxf(all, best), ref = now == -kInf ? 0.f : now;
+    const float old = __builtin_amdgcn_exp2f(all - ref);
+    const float f = live ? __builtin_amdgcn_exp2f(top - ref) : 0.f;
+    float part = live ? sum * f : 0.f;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) part += __shfl_xor(part, x);
+    total = total * old + part;
+    o *= old;
+    all = now;
+    const float* src = mine + first * step;
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) o += *reinterpret_cast<const f32x4*>(src + s * step) * __shfl(f, s);
   }
   const float inv = total != 0.f ? 1.f / total : 0.f;
-  if (d < dim) store4((T*)a.out + (int64_t)row * a.o_row + head * a.o_head + d, o * inv);
+  if (lane * 4 < dim) store4((T*)a.out + (int64_t)row * a.o_row + head * a.o_head + d, o * inv);
   if (lane == 0) a.lse[at] = (all + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
-template <typename T, int DT, int QT>
+template <typename T, int DT, int QT, bool kWhole>
 hipError_t launch(const AttentionArgs& a, hipStream_t stream) {
-  const dim3 grid((unsigned)slot_count(a), a.c.heads, a.splits);
-  attention_kernel<T, DT, QT><<<grid, kWaves * 64, 0, stream>>>(a);
+  const int64_t jobs = slot_count(a) * a.splits;
+  const dim3 grid((unsigned)((jobs + 7) / 8 * 8 * a.c.heads));
+  attention_kernel<T, DT, QT, kWhole><<<grid, kWaves * 64, 0, stream>>>(a);
   if (hipError_t e = hipGetLastError()) return e;
   if (a.splits > 1) {
     const int64_t rows = (int64_t)a.c.rows * a.q_heads;
@@ -408,18 +438,23 @@ hipError_t launch(const AttentionArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename T, int DT>
+template <typename T, int DT, bool kWhole>
 hipError_t by_rows(const AttentionArgs& a, hipStream_t stream) {
   if constexpr (DT <= 8)
-    if (a.row_tile == 32) return launch<T, DT, 2>(a, stream);
-  return launch<T, DT, 1>(a, stream);
+    if (a.row_tile == 32) return launch<T, DT, 2, kWhole>(a, stream);
+  return launch<T, DT, 1, kWhole>(a, stream);
+}
+
+template <typename T, int DT>
+hipError_t by_width(const AttentionArgs& a, hipStream_t stream) {
+  return a.c.dim == DT * 16 ? by_rows<T, DT, true>(a, stream) : by_rows<T, DT, false>(a, stream);
 }
 
 template <typename T>
 hipError_t by_dim(const AttentionArgs& a, hipStream_t stream) {
-  if (a.c.dim <= 64) return by_rows<T, 4>(a, stream);
-  if (a.c.dim <= 128) return by_rows<T, 8>(a, stream);
-  return by_rows<T, 16>(a, stream);
+  if (a.c.dim <= 64) return by_width<T, 4>(a, stream);
+  if (a.c.dim <= 128) return by_width<T, 8>(a, stream);
+  return by_width<T, 16>(a, stream);
 }
 
 }  // namespace
@@ -431,12 +466,15 @@ int64_t plan_attention(AttentionArgs& a, int64_t max_seq_len) {
   const int64_t slots = slot_count(a);
   int64_t longest = max_seq_len > 0 ? max_seq_len : 1;
   if (a.window && longest > a.window + kTile + per_seq) longest = a.window + kTile + per_seq;
-  // enough workgroups to fill the card several times over, of at least one
-  // tile a wave
-  const int64_t target = 4096, unit = kTile * kWaves;
+  // Four rounds of workgroups on the card (2 fit a compute unit) even out their
+  // lengths; more only add their beginnings and ends (64 contexts of 8-16k
+  // tokens: 285 us with 2048, 302 with 4096, 326 with 8192). Chunks are two
+  // tiles a wave at least, and a context of four or fewer is not split, since a
+  // join takes 3.5 us and its launch.
+  const int64_t target = 2048, unit = kTile * kWaves, least = 2 * unit;
   const int64_t work = slots * a.c.heads;
-  int64_t splits = target / (work > 0 ? work : 1);
-  const int64_t most = (longest + unit - 1) / unit;
+  int64_t splits = longest <= 2 * least ? 1 : target / (work > 0 ? work : 1);
+  const int64_t most = (longest + least - 1) / least;
   splits = splits < 1 ? 1 : splits > most ? most : splits;
   if (splits > 256) splits = 256;
   a.chunk = (int)(((longest + splits - 1) / splits + unit - 1) / unit * unit);

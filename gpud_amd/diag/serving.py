@@ -317,6 +317,8 @@ def cache_append(
     heads, dim, batch = cache[9], cache[11], cache[12]
     if tuple(k.shape) != (rows, heads, dim) or tuple(v.shape) != (rows, heads, dim):
         raise ValueError(f"k and v must be [T, {heads}, {dim}], not {tuple(k.shape)} and {tuple(v.shape)}")
+    if rows * heads > _INT_MAX // 2:
+        raise ValueError("more than 2^30 new keys")
     _check_gpu(device)
     if k.stride(2) != 1:
         k = k.contiguous()

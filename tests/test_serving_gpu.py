@@ -213,7 +213,7 @@ def same_codes(a, b):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
-@pytest.mark.parametrize("heads,dim,page", [(1, 16, 16), (2, 64, 16), (3, 80, 32), (2, 128, 64), (1, 256, 128)])
+@pytest.mark.parametrize("heads,dim,page", [(1, 16, 16), (2, 64, 16), (3, 80, 32), (2, 128, 64), (1, 256, 128), (1, 16, 512), (2, 64, 256)])
 def test_cache_append_in_steps(serving, heads, dim, page, dtype):
     """Prompts, chunks that end inside pages, and single tokens, each of another size."""
     g = gen(dim + page)

@@ -3,9 +3,8 @@
 //
 // Bound by one read of the logits. A wave takes a span of consecutive logits
 // in registers, finds their largest m, and then, with u = (x - m) log2 e, sums
-// 2^u and 2^u u and counts x > x_t. (The difference comes first: x log2 e alone
-// would leave fp32's range where a mask is the type's lowest value.) On the way it leaves the largest of each 64 consecutive logits (one
-// 128-byte line of 16-bit ones): no other trace of the alternatives is needed,
+// 2^u and 2^u u and counts x > x_t. On the way it leaves the largest of each 64
+// consecutive logits (one 128-byte line of 16-bit ones): no other trace of the alternatives is needed,
 // since the k best logits, by value and then by lower index, lie in the k best
 // spans by their largest and then by lower index, and in these in the k best
 // groups of 64. A second launch joins a row's spans in a fixed order and reads
@@ -60,8 +59,24 @@ __device__ __forceinline__ void unpack(u32x4 v, float* f, const float*) {
   for (int i = 0; i < 4; ++i) f[i] = bits_as<float>(v[i]);
 }
 
-// Larger of a lane's and its neighbour's; NaN gives way.
+// Larger of a lane's and another's; NaN gives way.
 __device__ __forceinline__ float max_xor(float v, int mask) { return fmaxf(v, __shfl_xor(v, mask)); }
+
+// Largest of kLanes neighbours (8 or 16), in all of them; NaN gives way. A step
+// is one instruction, whose second operand comes from the other lane.
+template <int kControl>
+__device__ __forceinline__ float max_dpp(float v) {
+  const int other = __builtin_amdgcn_update_dpp(0, bits_as<int>(v), kControl, 0xF, 0xF, true);
+  return fmaxf(v, bits_as<float>(other));
+}
+template <int kLanes>
+__device__ __forceinline__ float group_max(float v) {
+  v = max_dpp<0xB1>(v);   // lane ^ 1
+  v = max_dpp<0x4E>(v);   // lane ^ 2
+  v = max_dpp<0x141>(v);  // the other 4 of 8, mirrored
+  if constexpr (kLanes == 16) v = max_dpp<0x140>(v);  // the other 8 of 16, mirrored
+  return v;
+}
 
 // Whole numbers in the order of the values: -0 equals 0, NaN is above all.
 __device__ __forceinline__ uint32_t order_of(float f) {
@@ -69,9 +84,12 @@ __device__ __forceinline__ uint32_t order_of(float f) {
   const uint32_t b = bits_as<uint32_t>(f + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float value_of(uint32_t order) {
+  return bits_as<float>(order & 0x80000000u ? order & 0x7FFFFFFFu : ~order);  // all ones: NaN
+}
 
 template <typename T>
-__global__ __launch_bounds__(256) void spans_kernel(LogprobArgs a) {
+__global__ __launch_bounds__(256, 4) void spans_kernel(LogprobArgs a) {
   using S = Shape<T>;
   constexpr int V = S::kVec;
   const Layout lay(a.vocab, S::kSpan);
@@ -84,72 +102,109 @@ __global__ __launch_bounds__(256) void spans_kernel(LogprobArgs a) {
     const int first = span * S::kSpan + lane * V - shift;  // index of the lane's first value
 
     u32x4 raw[kUnits];
+    if (span * S::kSpan - shift >= 0 && (span + 1) * S::kSpan - shift <= a.vocab) {
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      const int e = first + u * 64 * V;
-      if (e >= 0 && e + V <= a.vocab) {
-        raw[u] = *reinterpret_cast<const u32x4*>(x + e);
-      } else {  // the row's ends: nothing outside it is read
-        T part[V];
+      for (int u = 0; u < kUnits; ++u) raw[u] = *reinterpret_cast<const u32x4*>(x + first + u * 64 * V);
+    } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) part[i] = (e + i >= 0 && e + i < a.vocab) ? x[e + i] : (T)-kInf;
-        __builtin_memcpy(&raw[u], part, 16);
+      for (int u = 0; u < kUnits; ++u) {
+        const int e = first + u * 64 * V;
+        if (e >= 0 && e + V <= a.vocab) {
+          raw[u] = *reinterpret_cast<const u32x4*>(x + e);
+        } else {  // the row's ends: nothing outside it is read
+          T part[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) part[i] = (e + i >= 0 && e + i < a.vocab) ? x[e + i] : (T)-kInf;
+          __builtin_memcpy(&raw[u], part, 16);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     const int64_t t = a.targets[row];
     const bool known = t >= 0 && t < a.vocab;
     const float xt = known ? (float)x[t] : kInf;
 
+    // The two passes over the registers unpack them anew: kept, the values
+    // would take the registers of three waves in five.
+    auto again = [&] {
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) asm volatile("" : "+v"(raw[u]));
+    };
     float best[kUnits];  // of the lane's group of 64 values
     float m = -kInf;
+    bool nan = false;
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       float f[V];
       unpack(raw[u], f, (const T*)nullptr);
       float b = f[0];
 #pragma unroll
-      for (int i = 1; i < V; ++i) b = fmaxf(b, f[i]);
-#pragma unroll
-      for (int d = 1; d < S::kLanes; d <<= 1) b = max_xor(b, d);
-      best[u] = b;
-      m = fmaxf(m, b);
+      for (int i = 1; i < V; ++i) b = __builtin_elementwise_maximum(b, f[i]);  // keeps a NaN
+      nan |= b != b;
+      best[u] = group_max<S::kLanes>(b);
+      m = fmaxf(m, best[u]);
     }
-#pragma unroll
-    for (int d = S::kLanes; d < 64; d <<= 1) m = max_xor(m, d);
+    if constexpr (S::kLanes == 8) m = max_dpp<0x140>(m);
+    m = max_xor(m, 16);
+    m = max_xor(m, 32);
+    const bool any_nan = __any(nan);
+    again();
 
     const float ref = m == -kInf ? 0.f : m;
     float sum = 0.f, weighted = 0.f;
     int above = 0;
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      float f[V];
-      unpack(raw[u], f, (const T*)nullptr);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float d = (f[i] - ref) * kLog2e;
-        const float p = __builtin_amdgcn_exp2f(d);
-        sum += p;
-        weighted = __builtin_fmaf(p, fmaxf(d, -256.f), weighted);  // 2^-256 is 0: no 0 x inf
-        above += __popcll(__ballot(f[i] > xt));
-      }
-    }
-    const bool odd = __any(sum != sum);  // a NaN or an infinity among the values
-    if (odd) {
-      float top = -kInf;
+    if (fabsf(ref) < 1e37f) {
+      // u = x log2 e - m log2 e in one step. The product with m is off by a
+      // rounding, the same for all values, and comes off the sums again; what
+      // lies below -1e38 (masks, -inf) is at 0 either way.
+      const float shift = ref * kLog2e, off = __builtin_fmaf(ref, kLog2e, -shift);
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         float f[V];
         unpack(raw[u], f, (const T*)nullptr);
-        bool nan = false;
 #pragma unroll
-        for (int i = 0; i < V; ++i) nan |= f[i] != f[i];
-        int any = nan;
+        for (int i = 0; i < V; ++i) {
+          const float d = __builtin_fmaf(fmaxf(f[i], -1e38f), kLog2e, -shift);
+          const float p = __builtin_amdgcn_exp2f(d);
+          sum += p;
+          weighted = __builtin_fmaf(p, d, weighted);
+          above += __popcll(__ballot(f[i] > xt));
+        }
+        __builtin_amdgcn_sched_barrier(0);  // registers
+      }
+      const float back = __builtin_amdgcn_exp2f(-off);
+      weighted = (weighted - off * sum) * back;
+      sum *= back;
+      if (m == -kInf) sum = weighted = 0.f;
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        float f[V];
+        unpack(raw[u], f, (const T*)nullptr);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float d = (f[i] - ref) * kLog2e;
+          const float p = __builtin_amdgcn_exp2f(d);
+          sum += p;
+          weighted = __builtin_fmaf(p, fmaxf(d, -256.f), weighted);  // 2^-256 is 0: no 0 x inf
+          above += __popcll(__ballot(f[i] > xt));
+        }
+      }
+    }
+    if (any_nan) {
+      again();
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        float f[V];
+        unpack(raw[u], f, (const T*)nullptr);
+        int any = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) any |= f[i] != f[i];
 #pragma unroll
         for (int d = 1; d < S::kLanes; d <<= 1) any |= __shfl_xor(any, d);
         if (any) best[u] = __builtin_nanf("");
-        if (__any(nan)) top = __builtin_nanf("");
       }
-      if (top != top) m = top;
+      m = sum = __builtin_nanf("");
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -184,25 +239,55 @@ __device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t place) {
   return (uint64_t)order << 32 | (uint32_t)~place;
 }
 
+__device__ __forceinline__ uint64_t shfl64(uint64_t v, int lane) {
+  const uint32_t lo = __shfl((uint32_t)v, lane), hi = __shfl((uint32_t)(v >> 32), lane);
+  return (uint64_t)hi << 32 | lo;
+}
+
 // Sorts out the `want` largest of list[0..n), all different, into out[0..want)
-// in falling order. The wave works alone.
-__device__ void select_top(const uint64_t* list, int n, int want, uint64_t* out, int lane) {
-  uint64_t floor_key = 0;  // keys from here on are the `want` largest
-  if (n > 256 && n > want) {
-    // the want-th largest by its bits, from the top: exact, for any list
-    for (int bit = 63; bit >= 0; --bit) {
-      const uint64_t trial = floor_key | 1ull << bit;
-      int count = 0;
-      for (int i = lane; i < n; i += 64) count += list[i] >= trial;
+// in falling order; list is used up. The wave works alone.
+__device__ void select_top(uint64_t* list, int n, int want, uint64_t* out, int lane) {
+  if (n > 64) {
+    // The want-th largest of the lanes' largest is a floor under the want
+    // largest of all, and seldom far under them.
+    uint64_t mine = 0;
+    for (int i = lane; i < n; i += 64) mine = list[i] > mine ? list[i] : mine;
+    int place = 0;
+#pragma unroll 8
+    for (int j = 0; j < 64; ++j) place += shfl64(mine, j) > mine;
+    uint64_t low = shfl64(mine, __ffsll((unsigned long long)__ballot(place == want - 1)) - 1);
+    auto keep = [&] {
+      int kept = 0;
+      for (int i = 0; i < n; i += 64) {
+        const uint64_t key = i + lane < n ? list[i + lane] : 0;
+        const bool in = i + lane < n && key >= low;
+        const uint64_t mask = __ballot(in);
+        __syncthreads();
+        if (in) list[kept + __popcll(mask & ((1ull << lane) - 1))] = key;
+        kept += __popcll(mask);
+      }
+      __syncthreads();
+      n = kept;
+    };
+    keep();
+    if (n > 256) {  // the largest lie in few lanes: their want-th by its bits, from the top
+      uint64_t exact = 0;
+      for (int bit = 63; bit >= 0; --bit) {
+        const uint64_t trial = exact | 1ull << bit;
+        int count = 0;
+        for (int i = lane; i < n; i += 64) count += list[i] >= trial;
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) count += __shfl_xor(count, d);
-      if (count >= want) floor_key = trial;
+        for (int d = 1; d < 64; d <<= 1) count += __shfl_xor(count, d);
+        if (count >= want) exact = trial;
+      }
+      low = exact;
+      keep();
     }
   }
   for (int i = lane; i < n; i += 64) {
     const uint64_t key = list[i];
-    if (key < floor_key) continue;
     int place = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) place += list[j] > key;
     if (place < want) out[place] = key;
   }
@@ -271,23 +356,32 @@ __global__ __launch_bounds__(64) void rows_kernel(LogprobArgs a) {
     const int size = level == 1 ? S::kGroups : 64;
     const uint32_t least = parts == want ? (uint32_t)(out[level - 1][parts - 1] >> 32) : 0u;
     n = 0;
-    for (int p = 0; p < parts; ++p) {
-      const uint32_t part = ~(uint32_t)out[level - 1][p];
-      uint32_t order = 0;
-      uint32_t place = part * size + lane;
-      bool in = lane < size;
-      if (level == 1) {
-        if (in) order = order_of(lay.group(a.work, row, 0)[place]);
-      } else {
-        const int e = (int)place - shift;
-        in = e >= 0 && e < a.vocab;
-        place = (uint32_t)e;
-        if (in) order = order_of((float)x[e]);
+    constexpr int kBatch = 8;
+    for (int first = 0; first < parts; first += kBatch) {
+      uint32_t order[kBatch], place[kBatch];
+      bool in[kBatch];
+#pragma unroll
+      for (int q = 0; q < kBatch; ++q) {
+        const uint32_t part = ~(uint32_t)out[level - 1][first + q < parts ? first + q : parts - 1];
+        place[q] = part * size + lane;
+        in[q] = first + q < parts && lane < size;
+        float v = 0.f;
+        if (level == 1) {
+          if (in[q]) v = lay.group(a.work, row, 0)[place[q]];
+        } else {
+          place[q] -= shift;
+          in[q] = in[q] && place[q] < (uint32_t)a.vocab;
+          if (in[q]) v = (float)x[place[q]];
+        }
+        order[q] = order_of(v);
       }
-      in = in && order >= least;
-      const uint64_t mask = __ballot(in);
-      if (in) list[n + __popcll(mask & ((1ull << lane) - 1))] = key_of(order, place);
-      n += __popcll(mask);
+#pragma unroll
+      for (int q = 0; q < kBatch; ++q) {
+        const bool kept = in[q] && order[q] >= least;
+        const uint64_t mask = __ballot(kept);
+        if (kept) list[n + __popcll(mask & ((1ull << lane) - 1))] = key_of(order[q], place[q]);
+        n += __popcll(mask);
+      }
     }
     __syncthreads();
     got = n < want ? n : want;
@@ -295,9 +389,9 @@ __global__ __launch_bounds__(64) void rows_kernel(LogprobArgs a) {
     __syncthreads();
   }
   for (int i = lane; i < want; i += 64) {
-    const uint32_t id = ~(uint32_t)out[2][i];
-    a.top_ids[row * want + i] = id;
-    a.top_logprobs[row * want + i] = logp((float)x[id]);
+    const uint64_t key = out[2][i];
+    a.top_ids[row * want + i] = ~(uint32_t)key;
+    a.top_logprobs[row * want + i] = logp(value_of((uint32_t)(key >> 32)));
   }
 }
 

@@ -12,6 +12,7 @@
 
 #include "geometry.h"
 #include "serving.h"
+#include "step.h"
 
 namespace py = pybind11;
 using namespace serving;
@@ -244,6 +245,26 @@ std::vector<std::vector<int64_t>> append_places(const std::vector<int32_t>& star
   return got;
 }
 
+py::dict step(int device, int iters, uint32_t seed, double oracle_offset) {
+  if (iters <= 0 || iters > 100000) throw std::invalid_argument("iters");
+  StepResult r;
+  {
+    py::gil_scoped_release release;
+    r = run_step(device, iters, seed, oracle_offset);
+  }
+  py::dict d;
+  d["ms_per_step"] = r.ms;
+  d["gbps"] = r.gbps;
+  d["product_gbps"] = r.product_gbps;
+  d["attention_gbps"] = r.attention_gbps;
+  d["logprob_gbps"] = r.logprob_gbps;
+  d["checked"] = r.checked;
+  d["verified"] = r.failures == 0;
+  d["verify_failures"] = r.failures;
+  d["messages"] = r.messages;
+  return d;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_serving, m) {
@@ -254,6 +275,9 @@ PYBIND11_MODULE(_serving, m) {
   m.def("attention_plan", &attention_plan);
   m.def("cache_attention", &cache_attention);
   m.def("logprob_workspace", &logprob_workspace);
+  m.def("serving_step", &step, py::arg("device") = 0, py::arg("iters") = 20, py::arg("seed") = 1,
+        py::arg("oracle_offset") = 0.0,
+        "One token step of a synthetic served model, checked against host oracles; returns rates + verification");
   m.def("attention_places", &attention_places);
   m.def("append_places", &append_places);
   m.def("token_logprobs", &token_logprobs);

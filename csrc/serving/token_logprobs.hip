@@ -239,8 +239,8 @@ __device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t place) {
   return (uint64_t)order << 32 | (uint32_t)~place;
 }
 
-__device__ __forceinline__ uint64_t shfl64(uint64_t v, int lane) {
-  const uint32_t lo = __shfl((uint32_t)v, lane), hi = __shfl((uint32_t)(v >> 32), lane);
+__device__ __forceinline__ uint64_t of_lane(uint64_t v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane), hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), lane);
   return (uint64_t)hi << 32 | lo;
 }
 
@@ -253,9 +253,9 @@ __device__ void select_top(uint64_t* list, int n, int want, uint64_t* out, int l
     uint64_t mine = 0;
     for (int i = lane; i < n; i += 64) mine = list[i] > mine ? list[i] : mine;
     int place = 0;
-#pragma unroll 8
-    for (int j = 0; j < 64; ++j) place += shfl64(mine, j) > mine;
-    uint64_t low = shfl64(mine, __ffsll((unsigned long long)__ballot(place == want - 1)) - 1);
+#pragma unroll
+    for (int j = 0; j < 64; ++j) place += of_lane(mine, j) > mine;
+    uint64_t low = of_lane(mine, __ffsll((unsigned long long)__ballot(place == want - 1)) - 1);
     auto keep = [&] {
       int kept = 0;
       for (int i = 0; i < n; i += 64) {

@@ -481,6 +481,7 @@ def diagnose(
         for name in (
             "accelerator-amd-diag-mfma",
             "accelerator-amd-diag-bandwidth",
+            "accelerator-amd-diag-serving",
             "accelerator-amd-diag-fabric",
         ):
             comp = core.registry.get(name)

@@ -6,6 +6,8 @@ BASELINE.json names these as first-class new components):
 
   * accelerator-amd-diag-mfma       — CDNA4 MFMA bf16/fp8 stress (csrc/diag)
   * accelerator-amd-diag-bandwidth  — HBM3E triad + LDS sweep
+  * accelerator-amd-diag-serving    — one token step of a served model in 4 and
+    8 bits (csrc/serving): products, paged cache, attention, log probabilities
   * accelerator-amd-diag-fabric     — RCCL all-reduce / pairwise xGMI check
 
 All are RunMode=manual (reference custom-plugin RunModeTypeManual —
@@ -31,6 +33,7 @@ from ..base import CheckResult, GPUdInstance, TickerComponent
 
 NAME_MFMA = "accelerator-amd-diag-mfma"
 NAME_BANDWIDTH = "accelerator-amd-diag-bandwidth"
+NAME_SERVING = "accelerator-amd-diag-serving"
 NAME_FABRIC = "accelerator-amd-diag-fabric"
 
 # Per-board floors for a healthy MI355X (measured ceilings: bf16 MFMA
@@ -45,6 +48,7 @@ DEFAULT_GEMM_TFLOPS_FLOOR = 1000.0  # v7P asm-K-loop bf16 GEMM, ~1390-1490
 DEFAULT_GEMM_FP8_TFLOPS_FLOOR = 1400.0  # 8-phase MX-fp8 GEMM, measured ~1940
 DEFAULT_HBM_GBPS_FLOOR = 4500.0
 DEFAULT_LDS_TBPS_FLOOR = 60.0
+DEFAULT_SERVING_GBPS_FLOOR = 800.0  # a whole step, measured ~1570
 DEFAULT_XGMI_PAIR_GBPS_FLOOR = 30.0  # per direction, pairwise sendrecv
 
 
@@ -56,6 +60,12 @@ def _load_diag():
     from ...diag import _diag  # type: ignore[attr-defined]
 
     return _diag
+
+
+def _load_serving():
+    from ...diag import _serving  # type: ignore[attr-defined]
+
+    return _serving
 
 
 class _ManualDiagComponent(TickerComponent):
@@ -248,6 +258,73 @@ class BandwidthDiagComponent(_ManualDiagComponent):
         )
 
 
+class ServingDiagComponent(_ManualDiagComponent):
+    """Runs the serving-step operators on every GPU as a decode step does.
+
+    What streams and GEMMs leave out: 4- and 8-bit decoding, gathers by page
+    tables, exp and log units, wave reductions, joins of split work. Sampled
+    outputs are compared with 64-bit oracles on the host, and all outputs of two
+    runs with each other.
+    """
+
+    def __init__(self, inst: GPUdInstance):
+        super().__init__(inst)
+        self.gbps_floor = DEFAULT_SERVING_GBPS_FLOOR
+        self.iters = 50
+
+    @property
+    def name(self) -> str:
+        return NAME_SERVING
+
+    def check(self) -> CheckResult:
+        try:
+            ndev = int(_load_diag().device_info()["device_count"])
+            serving = _load_serving()
+        except Exception as e:
+            return self._ext_missing_result(e)
+        if ndev == 0:
+            return CheckResult(
+                self.name, reason="no HIP devices", run_mode=self.run_mode
+            )
+        failures, extra = [], {}
+        for dev in range(ndev):
+            res = serving.serving_step(device=dev, iters=self.iters)
+            extra[f"gpu{dev}.step_ms"] = f"{res['ms_per_step']:.3f}"
+            extra[f"gpu{dev}.step_gbps"] = f"{res['gbps']:.0f}"
+            extra[f"gpu{dev}.product_gbps"] = f"{res['product_gbps']:.0f}"
+            extra[f"gpu{dev}.attention_gbps"] = f"{res['attention_gbps']:.0f}"
+            extra[f"gpu{dev}.logprob_gbps"] = f"{res['logprob_gbps']:.0f}"
+            if not res["verified"]:
+                detail = "; ".join(res["messages"][:2])
+                failures.append(
+                    f"gpu{dev}: serving step numeric verification FAILED "
+                    f"(bad={res['verify_failures']}: {detail})"
+                )
+            if res["gbps"] < self.gbps_floor:
+                failures.append(
+                    f"gpu{dev}: serving step {res['gbps']:.0f} GB/s below floor "
+                    f"{self.gbps_floor:.0f}"
+                )
+        if failures:
+            return CheckResult(
+                self.name,
+                health=HealthStateType.UNHEALTHY,
+                reason="; ".join(failures),
+                extra_info=extra,
+                run_mode=self.run_mode,
+                suggested_actions=SuggestedActions(
+                    description="serving-step diagnostic failed",
+                    repair_actions=[RepairActionType.HARDWARE_INSPECTION],
+                ),
+            )
+        return CheckResult(
+            self.name,
+            reason=f"serving step verified on {ndev} GPU(s)",
+            extra_info=extra,
+            run_mode=self.run_mode,
+        )
+
+
 class FabricDiagComponent(_ManualDiagComponent):
     def __init__(self, inst: GPUdInstance):
         super().__init__(inst)
@@ -356,5 +433,6 @@ def init_funcs():
     return [
         lambda inst: MFMADiagComponent(inst),
         lambda inst: BandwidthDiagComponent(inst),
+        lambda inst: ServingDiagComponent(inst),
         lambda inst: FabricDiagComponent(inst),
     ]

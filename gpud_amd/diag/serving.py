@@ -58,6 +58,18 @@ def _stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def _fits(t, device: int, dtype, shape) -> bool:
+    """Whether a contiguous tensor is what a call needs; the checks below say why not."""
+    return (
+        type(t) is torch.Tensor
+        and t.dtype is dtype
+        and t.get_device() == device
+        and t.shape == shape
+        and t.is_contiguous()
+        and not t.requires_grad
+    )
+
+
 def _check_input(name: str, t: torch.Tensor, device: Optional[torch.device], dtypes, dim: int) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, not {type(t).__name__}")
@@ -172,11 +184,14 @@ def w4_matmul(
     if k < 1 or n < 1 or k > MAX_COLUMNS or n > _INT_MAX // 2 or m > 65535 * 16:
         raise ValueError(f"no product of {m} rows with weights [{n}, {k}]")
     tiles, groups = -(-n // 16), -(-k // group_size)
-    _check_input("codes", codes, device, (torch.uint8,), 4)
-    _check_shape("codes", codes, (tiles, -(-k // 128), 64, 16))
-    _check_input("scales", scales, device, (x.dtype,), 3)
-    _check_shape("scales", scales, (tiles, groups, 16))
-    if zeros is not None:
+    at = x.get_device()
+    if not _fits(codes, at, torch.uint8, (tiles, -(-k // 128), 64, 16)):
+        _check_input("codes", codes, device, (torch.uint8,), 4)
+        _check_shape("codes", codes, (tiles, -(-k // 128), 64, 16))
+    if not _fits(scales, at, x.dtype, (tiles, groups, 16)):
+        _check_input("scales", scales, device, (x.dtype,), 3)
+        _check_shape("scales", scales, (tiles, groups, 16))
+    if zeros is not None and not _fits(zeros, at, torch.uint8, (tiles, groups, 16)):
         _check_input("zeros", zeros, device, (torch.uint8,), 3)
         _check_shape("zeros", zeros, (tiles, groups, 16))
     if codes.data_ptr() % 16 or scales.data_ptr() % 8:
@@ -248,22 +263,25 @@ def _check_cache_sizes(pages: int, heads: int, page: int, dim: int) -> None:
 
 def _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start, device, rows):
     _check_input("k_cache", k_cache, device, _CODES, 4)
-    _check_input("v_cache", v_cache, device, _CODES, 4)
     pages, heads, page, dim = k_cache.shape
     _check_cache_sizes(pages, heads, page, dim)
     if not k_cache.is_contiguous():
         raise ValueError("k_cache must be contiguous")
-    _check_shape("v_cache", v_cache, (pages, heads, dim, page))
-    _check_input("k_scale", k_scale, device, (torch.float32,), 2)
-    _check_input("v_scale", v_scale, device, (torch.float32,), 2)
-    _check_shape("k_scale", k_scale, (pages, heads))
-    _check_shape("v_scale", v_scale, (pages, heads))
+    at = k_cache.get_device()
+    if not _fits(v_cache, at, k_cache.dtype, (pages, heads, dim, page)):
+        _check_input("v_cache", v_cache, device, _CODES, 4)
+        _check_shape("v_cache", v_cache, (pages, heads, dim, page))
+    for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if not _fits(scale, at, torch.float32, (pages, heads)):
+            _check_input(name, scale, device, (torch.float32,), 2)
+            _check_shape(name, scale, (pages, heads))
     _check_input("block_table", block_table, device, (torch.int32,), 2)
-    _check_input("seq_lens", seq_lens, device, (torch.int32,), 1)
     batch, blocks = block_table.shape
     if blocks > 1 and block_table.stride(1) != 1:
         raise ValueError("rows of block_table must be dense")
-    _check_shape("seq_lens", seq_lens, (batch,))
+    if not _fits(seq_lens, at, torch.int32, (batch,)):
+        _check_input("seq_lens", seq_lens, device, (torch.int32,), 1)
+        _check_shape("seq_lens", seq_lens, (batch,))
     if blocks * page > _INT_MAX:
         raise ValueError("block_table covers more than 2^31 - 1 positions")
     starts = 0
@@ -271,8 +289,9 @@ def _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query
         if rows != batch:
             raise ValueError(f"{rows} rows for {batch} sequences: give query_start, or one row for each sequence")
     else:
-        _check_input("query_start", query_start, device, (torch.int32,), 1)
-        _check_shape("query_start", query_start, (batch + 1,))
+        if not _fits(query_start, at, torch.int32, (batch + 1,)):
+            _check_input("query_start", query_start, device, (torch.int32,), 1)
+            _check_shape("query_start", query_start, (batch + 1,))
         starts = query_start.data_ptr()
     kp, vp = k_cache.data_ptr(), v_cache.data_ptr()
     if kp % 16 or vp % 16:

@@ -319,6 +319,7 @@ class Session:
     DIAG_COMPONENTS = (
         "accelerator-amd-diag-mfma",
         "accelerator-amd-diag-bandwidth",
+        "accelerator-amd-diag-serving",
         "accelerator-amd-diag-fabric",
     )
 

@@ -292,3 +292,64 @@ def test_new_cache_refuses_sizes():
     for bad in ((0, 1, 64, 16), (1, 0, 64, 16), (1, 1, 65, 16), (1, 1, 64, 20), (1, 1, 64, 8)):
         with pytest.raises(ValueError):
             serving.new_cache(*bad, device="cpu")
+
+
+# -- the diagnostic that runs them -------------------------------------------
+
+
+class FakeDiag:
+    def device_info(self):
+        return {"device_count": 2}
+
+
+class FakeServing:
+    def __init__(self, **change):
+        self.res = dict(
+            ms_per_step=0.1, gbps=1500.0, product_gbps=1400.0, attention_gbps=2000.0, logprob_gbps=100.0,
+            checked=10, verified=True, verify_failures=0, messages=[],
+        )
+        self.res.update(change)
+        self.devices = []
+
+    def serving_step(self, device, iters):
+        self.devices.append(device)
+        return self.res
+
+
+def run_component(monkeypatch, fake):
+    from gpud_amd.components.accelerator import diag as diag_mod
+    from gpud_amd.components.base import GPUdInstance
+
+    monkeypatch.setattr(diag_mod, "_load_diag", lambda: FakeDiag())
+    monkeypatch.setattr(diag_mod, "_load_serving", lambda: fake)
+    return diag_mod.ServingDiagComponent(GPUdInstance()).trigger_check()
+
+
+def test_serving_component_runs_every_gpu(monkeypatch):
+    fake = FakeServing()
+    cr = run_component(monkeypatch, fake)
+    assert cr.health == "Healthy" and fake.devices == [0, 1]
+    assert cr.extra_info["gpu1.step_gbps"] == "1500"
+
+
+@pytest.mark.parametrize(
+    "change,said",
+    [
+        (dict(verified=False, verify_failures=3, messages=["logits: 3 bytes differ between two runs"]), "3 bytes differ"),
+        (dict(gbps=10.0), "below floor"),
+    ],
+)
+def test_serving_component_reports_a_sick_gpu(monkeypatch, change, said):
+    cr = run_component(monkeypatch, FakeServing(**change))
+    assert cr.health == "Unhealthy" and said in cr.reason
+    assert cr.suggested_actions.repair_actions == ["HARDWARE_INSPECTION"]
+
+
+def test_serving_component_is_registered_and_diagnosed():
+    from gpud_amd.components.accelerator import diag as diag_mod
+    from gpud_amd.components.base import GPUdInstance
+    from gpud_amd.session.session import Session
+
+    names = [f(GPUdInstance()).name for f in diag_mod.init_funcs()]
+    assert diag_mod.NAME_SERVING in names
+    assert diag_mod.NAME_SERVING in Session.DIAG_COMPONENTS

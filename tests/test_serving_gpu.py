@@ -688,3 +688,36 @@ def test_inference_without_gradients_and_with(serving):
         serving.w4_matmul(x, codes, scales, out_features=16)
     with torch.no_grad():
         close(serving.w4_matmul(x, codes, scales, out_features=16), want, bound)
+
+
+# ---------------------------------------------------------------------------
+# the diagnostic
+# ---------------------------------------------------------------------------
+
+
+def test_serving_step_verifies_and_compares():
+    from gpud_amd.diag import _serving
+
+    for seed in (1, 2):
+        res = _serving.serving_step(iters=3, seed=seed)
+        assert res["verified"] and res["verify_failures"] == 0, res
+        assert res["checked"] > 1_000_000 and res["gbps"] > 0
+    wrong = _serving.serving_step(iters=1, oracle_offset=0.5)  # the oracle is off, on the host
+    assert not wrong["verified"] and wrong["verify_failures"] > 100 and wrong["messages"]
+    with pytest.raises(ValueError):
+        _serving.serving_step(iters=0)
+
+
+def test_serving_component_on_gpu():
+    from gpud_amd.apiv1.types import HealthStateType
+    from gpud_amd.bootstrap import build_core
+
+    core = build_core(in_memory_db=True, kmsg_writable=False, record_reboot=False)
+    try:
+        comp = core.registry.get("accelerator-amd-diag-serving")
+        assert comp is not None
+        cr = comp.trigger_check()
+        assert cr.health == HealthStateType.HEALTHY, f"{cr.reason} / {cr.error}"
+        assert float(cr.extra_info["gpu0.step_gbps"]) > 0
+    finally:
+        core.close()

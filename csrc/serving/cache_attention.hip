@@ -20,8 +20,8 @@
 // results): they are p vs over the largest p vs so far, so at most 1, and what
 // falls under fp16's range is under 2^-24 of the result. Sums are fp32.
 //
-// A workgroup's 4 waves take turns at tiles of 64 tokens and join in LDS. Long
-// contexts are split over workgroups in chunks of a fixed number of tokens,
+// Of few rows, a workgroup's 4 waves take turns at tiles of 64 tokens and join
+// in LDS; of many, they have rows of their own and share the tiles. Long contexts are split over workgroups in chunks of a fixed number of tokens,
 // whose results a second launch joins in their order.
 #include <type_traits>
 
@@ -376,6 +376,305 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
   }
 }
 
+// Many rows: 4 waves with 32 rows each share the tiles of 64 tokens. A wave
+// fetches and widens a quarter of a tile, in the order of the matrix
+// instruction's operands, into one half of the LDS while all work on the other.
+// So codes are read and widened once for 128 rows; a tile then costs a wave 32
+// LDS reads of 1 KB for 64 matrix instructions, about the same time each.
+template <int DT>
+struct Staged {
+  static constexpr int kKeys = DT * 2, kValues = DT * 2;  // operands of 1 KB
+  static constexpr int kHalf = (kKeys + kValues) * 64;    // in 16 bytes
+  static constexpr size_t kBytes = 2 * (size_t)kHalf * 16;
+};
+
+template <typename T, int DT, bool kWhole>
+__global__ __launch_bounds__(kWaves * 64, DT <= 8 ? 2 : 1) void attention_rows_kernel(AttentionArgs a) {
+  using x8 = typename Mat<T>::x8;
+  constexpr int KB = DT / 4, QT = 2, VQ = DT / kWaves;
+  extern __shared__ u32x4 staged[];
+  __shared__ int flagged;
+  const CacheArgs& c = a.c;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane & 15, g = lane >> 4;
+  const int group = a.q_heads / c.heads;
+  const int turn = blockIdx.x >> 3, h = turn % c.heads;
+  const int64_t job = (int64_t)(turn / c.heads) * 8 + (blockIdx.x & 7);
+  const int slots = (int)slot_count(a);
+  const int split = (int)(job / slots), slot = (int)(job - (int64_t)split * slots);
+  if (split >= a.splits) return;
+  Place p;
+  if (!place_of_slot(a, group, slot, p)) return;
+  if (split >= p.splits) return;
+
+  const int page = c.page, dim = kWhole ? DT * 16 : c.dim;
+  const int shift = 31 - __clz(page);
+  const int begin = (p.lo & ~(kTile - 1)) + split * a.chunk;
+  const int end = split == p.splits - 1 || begin + a.chunk > p.hi ? p.hi : begin + a.chunk;
+  const int32_t* table = c.table + (p.b < c.batch ? p.b * c.ldt : 0);
+
+  x8 q[QT][KB * 2];
+  int pos[QT], low[QT];
+  const int mine = wave * 32;  // the wave's first row of the tile
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int i = mine + t * 16 + r < p.rows ? mine + t * 16 + r : p.rows - 1;
+    const int tok = (p.local + i) / group, head = h * group + (p.local + i) % group;
+    pos[t] = p.len - p.count + tok;
+    low[t] = a.window ? pos[t] - a.window : -1;
+    const T* src = (const T*)a.q + (int64_t)(p.row0 + tok) * a.q_row + head * a.q_head;
+#pragma unroll
+    for (int k = 0; k < KB * 2; ++k) {
+      const int d = (k >> 1) * 64 + g * 16 + (k & 1) * 8;
+      q[t][k] = bits_as<x8>(u32x4{0, 0, 0, 0});
+      if (kWhole || d < dim) q[t][k] = *reinterpret_cast<const x8*>(src + d);
+    }
+  }
+  // what the wave's rows see: nothing for a wave without rows
+  const int last_row = mine + 31 < p.rows ? mine + 31 : p.rows - 1;
+  const int w_first = p.len - p.count + (p.local + mine) / group;
+  const int w_last = mine < p.rows ? p.len - p.count + (p.local + last_row) / group : -1;
+  const int w_low = a.window ? w_first - a.window : -1;  // positions up to it are seen by none
+
+  f32x4 acc[QT][DT];
+  float top[QT], sum[QT];
+  u32x4 kr[KB], vr[VQ];
+  float ks, vs, ks_next, vs_next;
+  bool known, known_next;
+  auto look_up = [&](int base, bool& is) {
+    const int blk = (base + g * 16) >> shift;
+    const int pid = table[blk < c.blocks ? blk : c.blocks - 1];
+    is = blk < c.blocks && (uint32_t)pid < (uint32_t)c.pages && !p.broken;
+    return (uint32_t)pid < (uint32_t)c.pages ? pid : 0;
+  };
+  // the wave's quarter: token rows m = wave of the keys, VQ tiles of dimensions
+  auto fetch = [&](int base, int pid) {
+    const int pid_k = __shfl(pid, (r >> 2) << 4);
+    const int tok = ((base + ((r >> 2) << 4)) & (page - 1)) + (r & 3) + wave * 4;
+    const uint8_t* key = c.k + (((int64_t)pid_k * c.heads + h) * page + tok) * dim;
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+      kr[k] = *reinterpret_cast<const u32x4*>(key + (kWhole || k * 64 + g * 16 < dim ? k * 64 + g * 16 : 0));
+    const uint8_t* value = c.v + (((int64_t)pid * c.heads + h) * dim + r) * page + ((base + g * 16) & (page - 1));
+#pragma unroll
+    for (int d = 0; d < VQ; ++d)
+      vr[d] = *reinterpret_cast<const u32x4*>(value + (kWhole || (wave * VQ + d) * 16 < dim ? wave * VQ + d : 0) * 16 * page);
+    const int64_t ph = (int64_t)pid * c.heads + h;
+    ks_next = c.k_scale[ph];
+    vs_next = c.v_scale[ph];
+  };
+
+  auto sweep = [&](auto careful) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      top[t] = -kInf;
+      sum[t] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    bool odd = false;
+    // Values that no row sees become 0; NaN among the others is told, and in the
+    // careful form taken out.
+    auto put = [&](int base, int half) {
+      u32x4* to = staged + half * Staged<DT>::kHalf;
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        to[((wave * KB + k) * 2) * 64 + lane] = bits_as<u32x4>(Codes<T>::widen(kr[k][0], kr[k][1]));
+        to[((wave * KB + k) * 2 + 1) * 64 + lane] = bits_as<u32x4>(Codes<T>::widen(kr[k][2], kr[k][3]));
+      }
+      to += Staged<DT>::kKeys * 64;
+      if (base + kTile > p.first + 1 || (a.window && base <= p.last - a.window)) {
+        const int tok0 = base + g * 16;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t keep = bytes_below(p.hi - tok0 - 4 * w) & ~bytes_below(p.lo - tok0 - 4 * w);
+#pragma unroll
+          for (int d = 0; d < VQ; ++d) {
+            vr[d][w] &= keep;
+            const uint32_t nan = nan_bytes(vr[d][w]);
+            odd |= nan != 0;
+            if constexpr (careful) vr[d][w] &= ~((nan >> 7) * 0xFFu);
+          }
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < VQ; ++d)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          to[((wave * VQ + d) * 2 + x) * 64 + lane] =
+              bits_as<u32x4>(Codes<_Float16>::widen(vr[d][2 * x], vr[d][2 * x + 1]));
+    };
+
+    if (begin < end) {
+      int pid = look_up(begin, known_next);
+      fetch(begin, pid);
+      int beyond = begin + kTile < end ? begin + kTile : begin;
+      bool known_beyond;
+      pid = look_up(beyond, known_beyond);
+      put(begin, 0);
+      ks = ks_next, vs = vs_next, known = known_next;
+      __syncthreads();
+      int half = 0;
+#pragma unroll 1
+      for (int base = begin; base < end; base += kTile, half ^= 1) {
+        const bool more = base + kTile < end;
+        fetch(beyond, pid);  // the last tile is fetched again and left
+        known_next = known_beyond;
+        const int next = beyond;
+        beyond = beyond + kTile < end ? beyond + kTile : beyond;
+        pid = look_up(beyond, known_beyond);
+        const u32x4* at = staged + half * Staged<DT>::kHalf + lane;
+
+        if (base <= w_last && base + kTile - 1 > w_low) {
+          const int tok0 = base + g * 16;
+          const float unit = known ? ks * a.scale * kLog2e : __builtin_nanf("");
+          const float weight = known && tok0 < end ? vs : 1.f;
+          const float vlog = __builtin_amdgcn_logf(weight);
+          f32x4 s[QT][4] = {};
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int k = 0; k < KB * 2; ++k) {
+              const x8 key = bits_as<x8>(at[(m * KB * 2 + k) * 64]);
+#pragma unroll
+              for (int t = 0; t < QT; ++t) s[t][m] = Mat<T>::mfma(key, q[t][k], s[t][m]);
+            }
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) s[t][m] *= unit;
+          if (base + kTile > w_first + 1 || (a.window && base <= w_last - a.window)) {
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+#pragma unroll
+              for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int j = tok0 + m * 4 + i;
+                  const bool in = (j <= pos[t]) & (j > low[t]);
+                  s[t][m][i] = in ? s[t][m][i] : -kInf;
+                }
+          }
+          f16x8 pw[QT][2];
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            float best = -kInf;
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) best = fmaxf(best, s[t][m][i]);
+            best += vlog;
+            best = fmaxf(best, __shfl_xor(best, 16));
+            best = fmaxf(best, __shfl_xor(best, 32));
+            const float now = fmaxf(top[t], best);
+            const float ref = now == -kInf ? 0.f : now;
+            if (__any(now != top[t])) {
+              const float f = __builtin_amdgcn_exp2f(top[t] - ref);
+              sum[t] *= f;
+#pragma unroll
+              for (int d = 0; d < DT; ++d) acc[t][d] *= f;
+            }
+            top[t] = now;
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float e = __builtin_amdgcn_exp2f(s[t][m][i] - ref);
+                sum[t] += e;
+                pw[t][m >> 1][(m & 1) * 4 + i] = (_Float16)(e * weight);
+              }
+          }
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const f16x8 v = bits_as<f16x8>(at[(Staged<DT>::kKeys + d * 2 + x) * 64]);
+#pragma unroll
+              for (int t = 0; t < QT; ++t) acc[t][d] = Mat<_Float16>::mfma(v, pw[t][x], acc[t][d]);
+            }
+          if constexpr (careful) {
+            // which rows see a NaN among this tile's values, from the page itself
+#pragma unroll 1
+            for (int d = 0; d < DT; ++d) {
+              if (d * 16 >= dim) break;
+              bool is;
+              const int here = look_up(base, is);
+              const u32x4 raw = *reinterpret_cast<const u32x4*>(
+                  c.v + (((int64_t)here * c.heads + h) * dim + d * 16 + r) * page + (tok0 & (page - 1)));
+              f32x4 hits[QT] = {};
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const uint32_t w0 = nan_bytes(raw[2 * x]) >> 7, w1 = nan_bytes(raw[2 * x + 1]) >> 7;
+                f16x8 bad;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  bad[i] = (_Float16)(float)(w0 >> (8 * i) & 1u);
+                  bad[4 + i] = (_Float16)(float)(w1 >> (8 * i) & 1u);
+                }
+#pragma unroll
+                for (int t = 0; t < QT; ++t) {
+                  f16x8 seen;
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) {
+                    const int j = tok0 + x * 8 + i;
+                    seen[i] = (j <= pos[t]) & (j > low[t]) ? (_Float16)1.f : (_Float16)0.f;
+                  }
+                  hits[t] = Mat<_Float16>::mfma(bad, seen, hits[t]);
+                }
+              }
+#pragma unroll
+              for (int dd = 0; dd < DT; ++dd)
+                if (dd == d)
+#pragma unroll
+                  for (int t = 0; t < QT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                      if (hits[t][i] > 0.f) acc[t][dd][i] = __builtin_nanf("");
+            }
+          }
+        }
+        if (more) put(next, half ^ 1);
+        ks = ks_next, vs = vs_next, known = known_next;
+        __syncthreads();
+      }
+    }
+    return odd;
+  };
+
+  if (threadIdx.x == 0) flagged = 0;
+  __syncthreads();
+  if (__any(sweep(std::false_type{})) && lane == 0) flagged = 1;
+  __syncthreads();
+  if (flagged) sweep(std::true_type{});
+
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    sum[t] += __shfl_xor(sum[t], 16);
+    sum[t] += __shfl_xor(sum[t], 32);
+    const int i = mine + t * 16 + r;
+    if (i >= p.rows) continue;
+    if (p.splits == 1) {
+      const int tok = (p.local + i) / group, head = h * group + (p.local + i) % group;
+      const float inv = sum[t] != 0.f ? 1.f / sum[t] : 0.f;
+      T* out = (T*)a.out + (int64_t)(p.row0 + tok) * a.o_row + head * a.o_head + g * 4;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+        if (kWhole || d * 16 < dim) store4(out + d * 16, acc[t][d] * inv);
+      if (g == 0) a.lse[(int64_t)(p.row0 + tok) * a.q_heads + head] = (top[t] + __builtin_amdgcn_logf(sum[t])) * kLn2;
+    } else {
+      float* to = a.work + (((int64_t)slot * c.heads + h) * a.splits + split) * a.row_tile * (dim + 2);
+      float* row = to + (int64_t)i * dim + g * 4;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+        if (kWhole || d * 16 < dim) *reinterpret_cast<f32x4*>(row + d * 16) = acc[t][d];
+      if (g == 0) {
+        to[(int64_t)a.row_tile * dim + 2 * i] = top[t];
+        to[(int64_t)a.row_tile * dim + 2 * i + 1] = sum[t];
+      }
+    }
+  }
+}
+
 // Joins the splits of a row: one wave a row, four dimensions a lane. Lane s has
 // split s's reference and sum (a pass for each 64 splits).
 template <typename T>
@@ -425,11 +724,25 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
   if (lane == 0) a.lse[at] = (all + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
-template <typename T, int DT, int QT, bool kWhole>
+constexpr int kManyRows = 128;
+
+template <typename T, int DT, bool kWhole>
 hipError_t launch(const AttentionArgs& a, hipStream_t stream) {
   const int64_t jobs = slot_count(a) * a.splits;
-  const dim3 grid((unsigned)((jobs + 7) / 8 * 8 * a.c.heads));
-  attention_kernel<T, DT, QT, kWhole><<<grid, kWaves * 64, 0, stream>>>(a);
+  const dim3 grid((unsigned)((jobs + 7) / 8 * 8 * a.c.heads)), block(kWaves * 64);
+  if (a.row_tile == kManyRows) {
+    auto kernel = attention_rows_kernel<T, DT, kWhole>;
+    constexpr size_t bytes = Staged<DT>::kBytes;
+    if (bytes > 65536 - 64) {
+      const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+      if (e != hipSuccess) return e;
+    }
+    kernel<<<grid, block, bytes, stream>>>(a);
+  } else if (DT <= 8 && a.row_tile == 32) {
+    attention_kernel<T, DT <= 8 ? DT : 8, 2, kWhole><<<grid, block, 0, stream>>>(a);
+  } else {
+    attention_kernel<T, DT, 1, kWhole><<<grid, block, 0, stream>>>(a);
+  }
   if (hipError_t e = hipGetLastError()) return e;
   if (a.splits > 1) {
     const int64_t rows = (int64_t)a.c.rows * a.q_heads;
@@ -438,16 +751,9 @@ hipError_t launch(const AttentionArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename T, int DT, bool kWhole>
-hipError_t by_rows(const AttentionArgs& a, hipStream_t stream) {
-  if constexpr (DT <= 8)
-    if (a.row_tile == 32) return launch<T, DT, 2, kWhole>(a, stream);
-  return launch<T, DT, 1, kWhole>(a, stream);
-}
-
 template <typename T, int DT>
 hipError_t by_width(const AttentionArgs& a, hipStream_t stream) {
-  return a.c.dim == DT * 16 ? by_rows<T, DT, true>(a, stream) : by_rows<T, DT, false>(a, stream);
+  return a.c.dim == DT * 16 ? launch<T, DT, true>(a, stream) : launch<T, DT, false>(a, stream);
 }
 
 template <typename T>
@@ -457,22 +763,19 @@ hipError_t by_dim(const AttentionArgs& a, hipStream_t stream) {
   return by_width<T, 16>(a, stream);
 }
 
-}  // namespace
-
-int64_t plan_attention(AttentionArgs& a, int64_t max_seq_len) {
-  const int group = a.q_heads / a.c.heads;
-  const int64_t per_seq = a.c.starts ? (int64_t)a.c.rows * group / (a.c.batch > 0 ? a.c.batch : 1) : group;
-  a.row_tile = per_seq > 16 && a.c.dim <= 128 ? 32 : 16;  // registers
-  const int64_t slots = slot_count(a);
-  int64_t longest = max_seq_len > 0 ? max_seq_len : 1;
+// Splits a pass's contexts; returns its floats of workspace.
+int64_t split(AttentionArgs& a, int64_t per_seq) {
+  const int64_t slots = slot_count(a), work = slots * a.c.heads;
+  int64_t longest = a.longest > 0 ? a.longest : 1;
   if (a.window && longest > a.window + kTile + per_seq) longest = a.window + kTile + per_seq;
   // Four rounds of workgroups on the card (2 fit a compute unit) even out their
   // lengths; more only add their beginnings and ends (64 contexts of 8-16k
   // tokens: 285 us with 2048, 302 with 4096, 326 with 8192). Chunks are two
   // tiles a wave at least, and a context of four or fewer is not split, since a
-  // join takes 3.5 us and its launch.
-  const int64_t target = 2048, unit = kTile * kWaves, least = 2 * unit;
-  const int64_t work = slots * a.c.heads;
+  // join takes 3.5 us and its launch. Where many rows share a workgroup, one
+  // round will do.
+  const int64_t unit = kTile * kWaves, least = 2 * unit;
+  const int64_t target = a.row_tile == kManyRows ? 512 : 2048;
   int64_t splits = longest <= 2 * least ? 1 : target / (work > 0 ? work : 1);
   const int64_t most = (longest + least - 1) / least;
   splits = splits < 1 ? 1 : splits > most ? most : splits;
@@ -482,8 +785,46 @@ int64_t plan_attention(AttentionArgs& a, int64_t max_seq_len) {
   return a.splits == 1 ? 0 : work * a.splits * a.row_tile * (a.c.dim + 2);
 }
 
-hipError_t launch_cache_attention(const AttentionArgs& a, hipStream_t stream) {
-  return a.dtype == kBF16 ? by_dim<__bf16>(a, stream) : by_dim<_Float16>(a, stream);
+}  // namespace
+
+AttentionPlan plan_attention(const AttentionArgs& all) {
+  AttentionPlan plan{};
+  const int group = all.q_heads / all.c.heads;
+  const int64_t rows = (int64_t)all.c.rows * group;
+  const int64_t mean = all.c.starts ? rows / (all.c.batch > 0 ? all.c.batch : 1) : group;
+  constexpr int kFew = 64;  // rows that waves with tokens of their own still serve better
+  auto add = [&](int row_tile, int few, int many, int64_t per_seq) {
+    AttentionArgs& a = plan.pass[plan.passes++];
+    a = all;
+    a.row_tile = row_tile;
+    a.few = few;
+    a.many = many;
+    a.fill_tail = all.fill_tail && plan.passes == 1;
+    a.work = all.work ? all.work + plan.floats : nullptr;
+    plan.floats += split(a, per_seq);
+  };
+  const int most = 0x7FFFFFFF;
+  const int pair = all.c.dim <= 128 ? 32 : 16;  // two tiles of rows, if registers allow
+  if (!all.c.starts) {
+    if (group > kFew) add(kManyRows, 0, most, mean);
+    else add(group > 16 ? pair : 16, 0, most, mean);
+  } else if (mean <= 16 || rows <= kFew) {
+    add(16, 0, most, mean);
+  } else {
+    add(pair, 0, kFew, kFew);
+    add(kManyRows, kFew, most, mean);
+  }
+  return plan;
+}
+
+hipError_t launch_cache_attention(const AttentionArgs& all, hipStream_t stream) {
+  const AttentionPlan plan = plan_attention(all);
+  for (int i = 0; i < plan.passes; ++i) {
+    const AttentionArgs& a = plan.pass[i];
+    const hipError_t e = a.dtype == kBF16 ? by_dim<__bf16>(a, stream) : by_dim<_Float16>(a, stream);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace serving

@@ -59,6 +59,12 @@ __host__ __device__ inline void fill_place(const AttentionArgs& a, int group, Pl
   p.splits = n < a.splits ? n : a.splits;
 }
 
+// Whether a pass takes a sequence of `count` tokens.
+__host__ __device__ inline bool takes(const AttentionArgs& a, int group, int count) {
+  const int64_t rows = (int64_t)count * group;
+  return rows > a.few && rows <= a.many;
+}
+
 // The tile of a slot; false if it has none.
 __host__ __device__ inline bool place_of_slot(const AttentionArgs& a, int group, int slot, Place& p) {
   const CacheArgs& c = a.c;
@@ -82,13 +88,13 @@ __host__ __device__ inline bool place_of_slot(const AttentionArgs& a, int group,
     p.tile = slot - p.b * per;
     p.count = 1;
   }
-  if (p.b == c.batch && !a.fill_tail) return false;
+  if (p.b == c.batch ? !a.fill_tail : !takes(a, group, p.count)) return false;
   fill_place(a, group, p);
   return true;
 }
 
 // The tile of a query row and head, the slot it had and its row in the tile;
-// false if no sequence has the row.
+// false if no sequence of this pass has the row.
 __host__ __device__ inline bool place_of_row(const AttentionArgs& a, int group, int row, int head, Place& p,
                                              int64_t& slot, int& index) {
   const CacheArgs& c = a.c;
@@ -109,6 +115,7 @@ __host__ __device__ inline bool place_of_row(const AttentionArgs& a, int group, 
     p.count = 1;
     slot = (int64_t)row * ((group + a.row_tile - 1 >> tile_shift(a)));
   }
+  if (!takes(a, group, p.count)) return false;
   const int local = (row - p.row0) * group + head % group;
   p.tile = local >> tile_shift(a);
   index = local - p.tile * a.row_tile;

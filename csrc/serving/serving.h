@@ -59,18 +59,25 @@ struct AttentionArgs {
   const void* q;          // [rows][q_heads][dim], last dimension dense
   void* out;              // [rows][q_heads][dim], last dimension dense
   float* lse;             // [rows][q_heads]
-  float* work;            // attention_workspace() floats, or null if 0
+  float* work;            // plan_attention() floats, or null if 0
   int64_t q_row, q_head, o_row, o_head;
   int q_heads, window;    // window 0: none
-  int splits, chunk;      // plan_attention()
-  int row_tile;           // rows (token, head) of one workgroup
   int fill_tail;          // rows behind the last sequence become 0 / -inf
   float scale;
   int dtype;
+  int64_t longest;        // longest sequence as far as known: steers the split
+  // of a pass, by plan_attention()
+  int splits, chunk;      // workgroups of a context, and the tokens of one
+  int row_tile;           // rows (token, head) of a workgroup
+  int few, many;          // takes the sequences with more than few, at most many rows
 };
-// Fills splits, chunk and row_tile from the sizes and the longest expected
-// sequence; returns the floats of workspace that the launch needs.
-int64_t plan_attention(AttentionArgs& a, int64_t max_seq_len);
+// Sequences with few rows and those with many take passes of their own.
+struct AttentionPlan {
+  AttentionArgs pass[2];
+  int passes;
+  int64_t floats;         // of workspace
+};
+AttentionPlan plan_attention(const AttentionArgs& a);
 hipError_t launch_cache_attention(const AttentionArgs& a, hipStream_t stream);
 
 // ---- log probabilities of given tokens ------------------------------------

@@ -115,9 +115,7 @@ void cache_append(int device, uintptr_t stream, const py::tuple& cache, uintptr_
   OnDevice::check(launch_cache_append(a, stream_of(stream)), "cache_append");
 }
 
-// (floats of workspace, splits, chunk, row_tile)
-py::tuple attention_plan(int rows, int batch, int heads, int q_heads, int dim, bool ragged, int window,
-                         int64_t max_seq_len) {
+int64_t attention_floats(int rows, int batch, int heads, int q_heads, int dim, bool ragged, int window, int64_t longest) {
   AttentionArgs a{};
   static const int32_t some = 0;
   a.c.rows = rows;
@@ -127,13 +125,13 @@ py::tuple attention_plan(int rows, int batch, int heads, int q_heads, int dim, b
   a.c.starts = ragged ? &some : nullptr;  // only whether it is there counts
   a.q_heads = q_heads;
   a.window = window;
-  const int64_t floats = plan_attention(a, max_seq_len);
-  return py::make_tuple(floats, a.splits, a.chunk, a.row_tile);
+  a.longest = longest;
+  return plan_attention(a).floats;
 }
 
 void cache_attention(int device, uintptr_t stream, const py::tuple& cache, uintptr_t q, int64_t q_row, int64_t q_head,
                      uintptr_t out, int64_t o_row, int64_t o_head, uintptr_t lse, uintptr_t work, int q_heads,
-                     int window, int splits, int chunk, int row_tile, bool fill_tail, float scale, int dtype) {
+                     int window, int64_t longest, bool fill_tail, float scale, int dtype) {
   AttentionArgs a{};
   a.c = cache_args(cache);
   a.q = ptr<void>(q);
@@ -146,9 +144,7 @@ void cache_attention(int device, uintptr_t stream, const py::tuple& cache, uintp
   a.work = ptr<float>(work);
   a.q_heads = q_heads;
   a.window = window;
-  a.splits = splits;
-  a.chunk = chunk;
-  a.row_tile = row_tile;
+  a.longest = longest;
   a.fill_tail = fill_tail;
   a.scale = scale;
   a.dtype = dtype;
@@ -183,41 +179,45 @@ void token_logprobs(int device, uintptr_t stream, uintptr_t logits, int64_t ld, 
 std::vector<std::vector<int64_t>> attention_places(const std::vector<int32_t>& starts, const std::vector<int32_t>& lens,
                                                    int rows, int heads, int q_heads, int page, int blocks, int window,
                                                    int64_t max_seq_len, bool fill_tail) {
-  AttentionArgs a{};
-  a.c.starts = starts.empty() ? nullptr : starts.data();
-  a.c.lens = lens.data();
-  a.c.batch = (int)lens.size();
-  a.c.rows = rows;
-  a.c.heads = heads;
-  a.c.page = page;
-  a.c.blocks = blocks;
-  a.c.dim = 128;
-  a.q_heads = q_heads;
-  a.window = window;
-  a.fill_tail = fill_tail;
-  plan_attention(a, max_seq_len);
+  AttentionArgs all{};
+  all.c.starts = starts.empty() ? nullptr : starts.data();
+  all.c.lens = lens.data();
+  all.c.batch = (int)lens.size();
+  all.c.rows = rows;
+  all.c.heads = heads;
+  all.c.page = page;
+  all.c.blocks = blocks;
+  all.c.dim = 128;
+  all.q_heads = q_heads;
+  all.window = window;
+  all.fill_tail = fill_tail;
+  all.longest = max_seq_len;
   const int group = q_heads / heads;
   bool rising = true;
   for (size_t b = 0; b + 1 < starts.size(); ++b) rising &= starts[b] <= starts[b + 1];
   std::vector<std::vector<int64_t>> got;
-  for (int64_t slot = 0; slot < slot_count(a); ++slot) {
-    Place p;
-    if (!place_of_slot(a, group, (int)slot, p)) continue;
-    for (int split = 0; split < p.splits; ++split) {
-      const int begin = (p.lo & ~(kTile - 1)) + split * a.chunk;
-      const int end = split == p.splits - 1 || begin + a.chunk > p.hi ? p.hi : begin + a.chunk;
-      for (int i = 0; i < p.rows; ++i)
-        got.push_back({p.row0 + (p.local + i) / group, (p.local + i) % group, slot, split, begin, end});
-    }
-    for (int i = 0; i < p.rows && p.b < a.c.batch; ++i) {
-      Place again;
-      int64_t other;
-      int index;
-      const bool found = place_of_row(a, group, p.row0 + (p.local + i) / group, (p.local + i) % group, again, other, index);
-      const bool inside = !found || (other >= 0 && other < slot_count(a) && index >= 0 && index < a.row_tile &&
-                                     again.splits >= 1 && again.splits <= a.splits);
-      if (!inside || (rising && (!found || other != slot || index != i || again.splits != p.splits)))
-        throw std::runtime_error("a row's join looks elsewhere than its workgroup wrote");
+  const AttentionPlan plan = plan_attention(all);
+  for (int pass = 0; pass < plan.passes; ++pass) {
+    const AttentionArgs& a = plan.pass[pass];
+    for (int64_t slot = 0; slot < slot_count(a); ++slot) {
+      Place p;
+      if (!place_of_slot(a, group, (int)slot, p)) continue;
+      for (int split = 0; split < p.splits; ++split) {
+        const int begin = (p.lo & ~(kTile - 1)) + split * a.chunk;
+        const int end = split == p.splits - 1 || begin + a.chunk > p.hi ? p.hi : begin + a.chunk;
+        for (int i = 0; i < p.rows; ++i)
+          got.push_back({p.row0 + (p.local + i) / group, (p.local + i) % group, slot, split, begin, end});
+      }
+      for (int i = 0; i < p.rows && p.b < a.c.batch; ++i) {
+        Place again;
+        int64_t other;
+        int index;
+        const bool found = place_of_row(a, group, p.row0 + (p.local + i) / group, (p.local + i) % group, again, other, index);
+        const bool inside = !found || (other >= 0 && other < slot_count(a) && index >= 0 && index < a.row_tile &&
+                                       again.splits >= 1 && again.splits <= a.splits);
+        if (!inside || (rising && (!found || other != slot || index != i || again.splits != p.splits)))
+          throw std::runtime_error("a row's join looks elsewhere than its workgroup wrote");
+      }
     }
   }
   return got;
@@ -272,7 +272,7 @@ PYBIND11_MODULE(_serving, m) {
   m.def("w4_workspace", &w4_work);
   m.def("w4_matmul", &w4_matmul);
   m.def("cache_append", &cache_append);
-  m.def("attention_plan", &attention_plan);
+  m.def("attention_workspace", &attention_floats);
   m.def("cache_attention", &cache_attention);
   m.def("logprob_workspace", &logprob_workspace);
   m.def("serving_step", &step, py::arg("device") = 0, py::arg("iters") = 20, py::arg("seed") = 1,

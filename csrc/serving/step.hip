@@ -271,7 +271,8 @@ StepResult run_step(int device, int iters, uint32_t seed, double oracle_offset) 
   attention.q_heads = kQHeads;
   attention.scale = 1.f / std::sqrt((float)kDim);
   attention.dtype = kBF16;
-  Buffer split(plan_attention(attention, kLongest) * 4);
+  attention.longest = kLongest;
+  Buffer split(plan_attention(attention).floats * 4);
   attention.work = split.as<float>();
 
   std::vector<int64_t> targets(kBatch);

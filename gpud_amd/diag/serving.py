@@ -420,14 +420,15 @@ def cache_attention(
             out.zero_()
         lse.fill_(-math.inf)
         return out, lse
-    floats, splits, chunk, row_tile = _serving.attention_plan(
-        rows, batch, heads, q_heads, dim, query_start is not None, min(window or 0, _INT_MAX // 2), max_seq_len
+    window = min(window or 0, _INT_MAX // 2)
+    floats = _serving.attention_workspace(
+        rows, batch, heads, q_heads, dim, query_start is not None, window, max_seq_len
     )
     work = torch.empty(floats, dtype=torch.float32, device=device) if floats else None
     _serving.cache_attention(
         device.index, _stream(device), cache, q.data_ptr(), q.stride(0), q.stride(1),
         out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), work.data_ptr() if floats else 0,
-        q_heads, min(window or 0, _INT_MAX // 2), splits, chunk, row_tile, fill, scale, _DTYPES[q.dtype],
+        q_heads, window, max_seq_len, fill, scale, _DTYPES[q.dtype],
     )
     return out, lse
 

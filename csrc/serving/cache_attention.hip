@@ -75,6 +75,19 @@ __device__ __forceinline__ void store4(T* to, f32x4 v) {
   *reinterpret_cast<t4*>(to) = r;
 }
 
+// How a lane's 16 tokens, all of one page, weigh in: a score's power of two is
+// unit q . K + log, with the value's scale in it, and `back` takes that out of
+// the sum again.
+struct Weighing {
+  float unit, log, back;
+  __device__ __forceinline__ Weighing(bool known, bool within, float ks, float vs, float scale) {
+    unit = known ? ks * scale * kLog2e : __builtin_nanf("");
+    const float v = known && within ? vs : 1.f;
+    log = __builtin_amdgcn_logf(v);
+    back = 1.f / v;
+  }
+};
+
 // DT tiles of 16 dimensions, all of them there if kWhole; QT tiles of 16 query
 // rows.
 // Codes that one workgroup reads once pass by the L2.
@@ -191,9 +204,7 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
     for (; base < end; base += kWaves * kTile) {
       const int tok0 = base + g * 16;  // the lane's 16 tokens for P and V
       load_values(base, here);
-      const float unit = here.known ? ks * a.scale * kLog2e : __builtin_nanf("");
-      const float weight = here.known && tok0 < end ? vs : 1.f;
-      const float vlog = __builtin_amdgcn_logf(weight);
+      Weighing by(here.known, tok0 < end, ks, vs, a.scale);
 
       f32x4 s[QT][4] = {};
 #pragma unroll
@@ -212,10 +223,6 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
       here = next;
       next = look_up(ahead + kWaves * kTile < end ? ahead + kWaves * kTile : ahead);
 
-#pragma unroll
-      for (int t = 0; t < QT; ++t)
-#pragma unroll
-        for (int m = 0; m < 4; ++m) s[t][m] *= unit;
       const bool edge = base + kTile > p.first + 1 || (a.window && base <= p.last - a.window);
       if (edge) {
 #pragma unroll
@@ -226,8 +233,9 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
             for (int i = 0; i < 4; ++i) {
               const int j = tok0 + m * 4 + i;
               const bool in = (j <= pos[t]) & (j > low[t]);
-              s[t][m][i] = in ? s[t][m][i] : -kInf;
+              s[t][m][i] = in ? s[t][m][i] * by.unit : -kInf;
             }
+        by.unit = 1.f;  // masked behind the unit: an unknown page's NaN stays with the rows that see it
       }
       f16x8 pw[QT][2];
 #pragma unroll
@@ -237,26 +245,30 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
         for (int m = 0; m < 4; ++m)
 #pragma unroll
           for (int i = 0; i < 4; ++i) best = fmaxf(best, s[t][m][i]);
-        best += vlog;
+        best = __builtin_fmaf(best, by.unit, by.log);
         best = fmaxf(best, __shfl_xor(best, 16));
         best = fmaxf(best, __shfl_xor(best, 32));
-        const float now = fmaxf(top[t], best);
-        const float ref = now == -kInf ? 0.f : now;
+        // the reference moves only where weights would leave 2^8: fp16 and fp32
+        // hold them as exactly there
+        const float now = best > top[t] + 8.f ? best : top[t];
         if (__any(now != top[t])) {
-          const float f = __builtin_amdgcn_exp2f(top[t] - ref);
+          const float f = now == -kInf ? 0.f : __builtin_amdgcn_exp2f(top[t] - now);
           sum[t] *= f;
 #pragma unroll
           for (int d = 0; d < DT; ++d) acc[t][d] *= f;
+          top[t] = now;
         }
-        top[t] = now;
+        const float off = by.log - (now == -kInf ? 0.f : now);
+        float part = 0.f;
 #pragma unroll
         for (int m = 0; m < 4; ++m)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float e = __builtin_amdgcn_exp2f(s[t][m][i] - ref);
-            sum[t] += e;
-            pw[t][m >> 1][(m & 1) * 4 + i] = (_Float16)(e * weight);
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][m][i], by.unit, off));
+            part += e;
+            pw[t][m >> 1][(m & 1) * 4 + i] = (_Float16)e;
           }
+        sum[t] = __builtin_fmaf(part, by.back, sum[t]);
       }
       if (edge) {
         // values that no row sees are whatever the page held before
@@ -527,9 +539,7 @@ __global__ __launch_bounds__(kWaves * 64, DT <= 8 ? 2 : 1) void attention_rows_k
 
         if (base <= w_last && base + kTile - 1 > w_low) {
           const int tok0 = base + g * 16;
-          const float unit = known ? ks * a.scale * kLog2e : __builtin_nanf("");
-          const float weight = known && tok0 < end ? vs : 1.f;
-          const float vlog = __builtin_amdgcn_logf(weight);
+          Weighing by(known, tok0 < end, ks, vs, a.scale);
           f32x4 s[QT][4] = {};
 #pragma unroll
           for (int m = 0; m < 4; ++m)
@@ -539,10 +549,6 @@ __global__ __launch_bounds__(kWaves * 64, DT <= 8 ? 2 : 1) void attention_rows_k
 #pragma unroll
               for (int t = 0; t < QT; ++t) s[t][m] = Mat<T>::mfma(key, q[t][k], s[t][m]);
             }
-#pragma unroll
-          for (int t = 0; t < QT; ++t)
-#pragma unroll
-            for (int m = 0; m < 4; ++m) s[t][m] *= unit;
           if (base + kTile > w_first + 1 || (a.window && base <= w_last - a.window)) {
 #pragma unroll
             for (int t = 0; t < QT; ++t)
@@ -552,8 +558,9 @@ __global__ __launch_bounds__(kWaves * 64, DT <= 8 ? 2 : 1) void attention_rows_k
                 for (int i = 0; i < 4; ++i) {
                   const int j = tok0 + m * 4 + i;
                   const bool in = (j <= pos[t]) & (j > low[t]);
-                  s[t][m][i] = in ? s[t][m][i] : -kInf;
+                  s[t][m][i] = in ? s[t][m][i] * by.unit : -kInf;
                 }
+            by.unit = 1.f;
           }
           f16x8 pw[QT][2];
 #pragma unroll
@@ -563,26 +570,30 @@ __global__ __launch_bounds__(kWaves * 64, DT <= 8 ? 2 : 1) void attention_rows_k
             for (int m = 0; m < 4; ++m)
 #pragma unroll
               for (int i = 0; i < 4; ++i) best = fmaxf(best, s[t][m][i]);
-            best += vlog;
+            best = __builtin_fmaf(best, by.unit, by.log);
             best = fmaxf(best, __shfl_xor(best, 16));
             best = fmaxf(best, __shfl_xor(best, 32));
-            const float now = fmaxf(top[t], best);
-            const float ref = now == -kInf ? 0.f : now;
+            // the reference moves only where weights would leave 2^8: fp16 and fp32
+            // hold them as exactly there
+            const float now = best > top[t] + 8.f ? best : top[t];
             if (__any(now != top[t])) {
-              const float f = __builtin_amdgcn_exp2f(top[t] - ref);
+              const float f = now == -kInf ? 0.f : __builtin_amdgcn_exp2f(top[t] - now);
               sum[t] *= f;
 #pragma unroll
               for (int d = 0; d < DT; ++d) acc[t][d] *= f;
+              top[t] = now;
             }
-            top[t] = now;
+            const float off = by.log - (now == -kInf ? 0.f : now);
+            float part = 0.f;
 #pragma unroll
             for (int m = 0; m < 4; ++m)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const float e = __builtin_amdgcn_exp2f(s[t][m][i] - ref);
-                sum[t] += e;
-                pw[t][m >> 1][(m & 1) * 4 + i] = (_Float16)(e * weight);
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][m][i], by.unit, off));
+                part += e;
+                pw[t][m >> 1][(m & 1) * 4 + i] = (_Float16)e;
               }
+            sum[t] = __builtin_fmaf(part, by.back, sum[t]);
           }
 #pragma unroll
           for (int d = 0; d < DT; ++d)
@@ -675,53 +686,63 @@ __global__ __launch_bounds__(kWaves * 64, DT <= 8 ? 2 : 1) void attention_rows_k
   }
 }
 
-// Joins the splits of a row: one wave a row, four dimensions a lane. Lane s has
-// split s's reference and sum (a pass for each 64 splits).
-template <typename T>
+// Joins the splits of 16 rows of a slot and head, 16 lanes a row: lane j of them
+// has split j's reference and sum (a pass for each 16 splits) and the dimensions
+// 4 j .. + 3 of each 64.
+template <typename T, int kParts>
 __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
   const CacheArgs& c = a.c;
-  const int lane = threadIdx.x & 63;
-  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= (int64_t)c.rows * a.q_heads) return;
-  const int row = (int)(at / a.q_heads), head = (int)(at % a.q_heads);
-  const int group = a.q_heads / c.heads, h = head / group, dim = c.dim;
+  const int lane = threadIdx.x & 63, j = lane & 15, dim = c.dim;
+  const int group = a.q_heads / c.heads, pieces = a.row_tile / 16;
+  const int piece = blockIdx.x % pieces;
+  const int job = blockIdx.x / pieces, h = job % c.heads, slot = job / c.heads;
   Place p;
-  int64_t slot;
-  int i;
-  if (!place_of_row(a, group, row, head, p, slot, i)) return;
-  if (p.splits == 1) return;  // written whole
+  if (!place_of_slot(a, group, slot, p)) return;
+  if (p.splits == 1 || piece * 16 >= p.rows) return;  // written whole, or nothing there
+  const int row = piece * 16 + (threadIdx.x >> 4);
+  const bool live = row < p.rows;
+  const int i = live ? row : p.rows - 1;
 
-  const float* from = a.work + (slot * c.heads + h) * a.splits * a.row_tile * (dim + 2);
   const int64_t step = (int64_t)a.row_tile * (dim + 2);
+  const float* from = a.work + ((int64_t)slot * c.heads + h) * a.splits * step;
   const float* heads = from + (int64_t)a.row_tile * dim + 2 * i;
-  const int d = lane * 4 < dim ? lane * 4 : 0;
-  const float* mine = from + (int64_t)i * dim + d;
+  const float* mine = from + (int64_t)i * dim + j * 4;
   float all = -kInf, total = 0.f;
-  f32x4 o = {};
-  for (int first = 0; first < p.splits; first += 64) {
-    const int n = p.splits - first < 64 ? p.splits - first : 64;
-    const float* at64 = heads + (first + (lane < n ? lane : 0)) * step;
-    const float top = at64[0], sum = at64[1];
-    const bool live = lane < n;
-    float best = live ? top : -kInf;
+  f32x4 o[kParts] = {};
+  for (int first = 0; first < p.splits; first += 16) {
+    const int n = p.splits - first < 16 ? p.splits - first : 16;
+    const float* at = heads + (first + (j < n ? j : 0)) * step;
+    const float top = at[0], sum = at[1];
+    float best = j < n ? top : -kInf;
 #pragma unroll
-    for (int x = 1; x < 64; x <<= 1) best = fmaxf(best, __shfl_xor(best, x));
+    for (int x = 1; x < 16; x <<= 1) best = fmaxf(best, __shfl_xor(best, x));
     const float now = fmaxf(all, best), ref = now == -kInf ? 0.f : now;
     const float old = __builtin_amdgcn_exp2f(all - ref);
-    const float f = live ? __builtin_amdgcn_exp2f(top - ref) : 0.f;
-    float part = live ? sum * f : 0.f;
+    const float f = j < n ? __builtin_amdgcn_exp2f(top - ref) : 0.f;
+    float part = j < n ? sum * f : 0.f;
 #pragma unroll
-    for (int x = 1; x < 64; x <<= 1) part += __shfl_xor(part, x);
+    for (int x = 1; x < 16; x <<= 1) part += __shfl_xor(part, x);
     total = total * old + part;
-    o *= old;
     all = now;
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) o[q] *= old;
     const float* src = mine + first * step;
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) o += *reinterpret_cast<const f32x4*>(src + s * step) * __shfl(f, s);
+#pragma unroll 2
+    for (int s = 0; s < n; ++s) {
+      const float w = __shfl(f, (lane & 48) + s);
+#pragma unroll
+      for (int q = 0; q < kParts; ++q)
+        if (q * 64 + j * 4 < dim) o[q] += *reinterpret_cast<const f32x4*>(src + s * step + q * 64) * w;
+    }
   }
+  if (!live) return;
+  const int tok = (p.local + i) / group, head = h * group + (p.local + i) % group;
   const float inv = total != 0.f ? 1.f / total : 0.f;
-  if (lane * 4 < dim) store4((T*)a.out + (int64_t)row * a.o_row + head * a.o_head + d, o * inv);
-  if (lane == 0) a.lse[at] = (all + __builtin_amdgcn_logf(total)) * kLn2;
+  T* out = (T*)a.out + (int64_t)(p.row0 + tok) * a.o_row + head * a.o_head + j * 4;
+#pragma unroll
+  for (int q = 0; q < kParts; ++q)
+    if (q * 64 + j * 4 < dim) store4(out + q * 64, o[q] * inv);
+  if (j == 0) a.lse[(int64_t)(p.row0 + tok) * a.q_heads + head] = (all + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
 constexpr int kManyRows = 128;
@@ -745,8 +766,7 @@ hipError_t launch(const AttentionArgs& a, hipStream_t stream) {
   }
   if (hipError_t e = hipGetLastError()) return e;
   if (a.splits > 1) {
-    const int64_t rows = (int64_t)a.c.rows * a.q_heads;
-    join_kernel<T><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, stream>>>(a);
+    join_kernel<T, DT / 4><<<dim3((unsigned)(slot_count(a) * a.c.heads * (a.row_tile / 16))), 256, 0, stream>>>(a);
   }
   return hipGetLastError();
 }
@@ -775,7 +795,7 @@ int64_t split(AttentionArgs& a, int64_t per_seq) {
   // join takes 3.5 us and its launch. Where many rows share a workgroup, one
   // round will do.
   const int64_t unit = kTile * kWaves, least = 2 * unit;
-  const int64_t target = a.row_tile == kManyRows ? 512 : 2048;
+  const int64_t target = a.row_tile == kManyRows ? 768 : 2048;
   int64_t splits = longest <= 2 * least ? 1 : target / (work > 0 ? work : 1);
   const int64_t most = (longest + least - 1) / least;
   splits = splits < 1 ? 1 : splits > most ? most : splits;
@@ -793,26 +813,27 @@ AttentionPlan plan_attention(const AttentionArgs& all) {
   const int64_t rows = (int64_t)all.c.rows * group;
   const int64_t mean = all.c.starts ? rows / (all.c.batch > 0 ? all.c.batch : 1) : group;
   constexpr int kFew = 64;  // rows that waves with tokens of their own still serve better
-  auto add = [&](int row_tile, int few, int many, int64_t per_seq) {
+  auto add = [&](int row_tile, int per, int few, int many, int64_t per_seq) {
     AttentionArgs& a = plan.pass[plan.passes++];
     a = all;
     a.row_tile = row_tile;
     a.few = few;
     a.many = many;
-    a.fill_tail = all.fill_tail && plan.passes == 1;
+    a.per = per;
+    a.fill_tail = all.fill_tail && per == 0;
     a.work = all.work ? all.work + plan.floats : nullptr;
     plan.floats += split(a, per_seq);
   };
   const int most = 0x7FFFFFFF;
   const int pair = all.c.dim <= 128 ? 32 : 16;  // two tiles of rows, if registers allow
   if (!all.c.starts) {
-    if (group > kFew) add(kManyRows, 0, most, mean);
-    else add(group > 16 ? pair : 16, 0, most, mean);
+    const int tile = group > kFew ? kManyRows : group > 16 ? pair : 16;
+    add(tile, (group + tile - 1) / tile, 0, most, mean);
   } else if (mean <= 16 || rows <= kFew) {
-    add(16, 0, most, mean);
+    add(16, 0, 0, most, mean);
   } else {
-    add(pair, 0, kFew, kFew);
-    add(kManyRows, kFew, most, mean);
+    add(pair, kFew / pair, 0, kFew, kFew);
+    add(kManyRows, 0, kFew, most, mean);
   }
   return plan;
 }

@@ -13,6 +13,30 @@ namespace serving {
 
 constexpr int kTile = 64;  // tokens that a wave takes at once
 
+// The last of 0 .. count - 1 whose first(i) is not over `at`; 0 if there is
+// none. first() does not fall. On the device all lanes of a wave ask for the
+// same: few places are counted at once, since each step of a search waits for
+// memory.
+template <typename First>
+__host__ __device__ inline int last_at_most(int count, int64_t at, First first) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  if (count <= 512) {
+    int found = 0;
+    for (int i = 0; i < count; i += 64) {
+      const int lane = i + (threadIdx.x & 63);
+      found += __popcll(__ballot(lane < count && first(lane < count ? lane : 0) <= at));
+    }
+    return found > 0 ? found - 1 : 0;
+  }
+#endif
+  int lo = 0, hi = count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first(mid) <= at) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
 // ---- attention -------------------------------------------------------------
 
 // Rows of a sequence are (token, head) pairs, `row_tile` of them a workgroup.
@@ -27,15 +51,16 @@ struct Place {
 // Rows of a tile are a power of two.
 __host__ __device__ inline int tile_shift(const AttentionArgs& a) { return __builtin_ctz(a.row_tile); }
 
-// Slots of sequence b start at starts[b] group / row_tile + b: enough for its
-// tiles, whatever the lengths, and a rule that a binary search can invert.
+// Where sequences have few rows, each has `per` slots. Otherwise those of
+// sequence b start at starts[b] group / row_tile + b: enough for its tiles,
+// whatever the lengths, and a rule that a search can invert.
 __host__ __device__ inline int64_t first_slot(const AttentionArgs& a, int group, int b) {
   return ((int64_t)a.c.starts[b] * group >> tile_shift(a)) + b;
 }
 
 __host__ __device__ inline int64_t slot_count(const AttentionArgs& a) {
   const int group = a.q_heads / a.c.heads;
-  if (!a.c.starts) return (int64_t)a.c.batch * ((group + a.row_tile - 1 >> tile_shift(a)));
+  if (a.per) return (int64_t)a.c.batch * a.per;
   return ((int64_t)a.c.rows * group >> tile_shift(a)) + a.c.batch + 1;
 }
 
@@ -59,6 +84,20 @@ __host__ __device__ inline void fill_place(const AttentionArgs& a, int group, Pl
   p.splits = n < a.splits ? n : a.splits;
 }
 
+// The rows of sequence p.b; false if it has none.
+__host__ __device__ inline bool rows_of(const CacheArgs& c, Place& p) {
+  if (!c.starts) {
+    p.row0 = p.b;
+    p.count = 1;
+    return p.b < c.rows;
+  }
+  p.row0 = c.starts[p.b];
+  const int next = p.b < c.batch ? c.starts[p.b + 1] : c.rows;
+  if (p.row0 < 0 || next <= p.row0 || next > c.rows) return false;
+  p.count = next - p.row0;
+  return true;
+}
+
 // Whether a pass takes a sequence of `count` tokens.
 __host__ __device__ inline bool takes(const AttentionArgs& a, int group, int count) {
   const int64_t rows = (int64_t)count * group;
@@ -68,58 +107,18 @@ __host__ __device__ inline bool takes(const AttentionArgs& a, int group, int cou
 // The tile of a slot; false if it has none.
 __host__ __device__ inline bool place_of_slot(const AttentionArgs& a, int group, int slot, Place& p) {
   const CacheArgs& c = a.c;
-  if (c.starts) {
-    int lo = 0, hi = c.batch + 1;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (first_slot(a, group, mid) <= slot) lo = mid; else hi = mid;
-    }
-    p.b = lo;
-    p.row0 = c.starts[lo];
-    const int next = lo < c.batch ? c.starts[lo + 1] : c.rows;
-    if (p.row0 < 0 || next <= p.row0 || next > c.rows) return false;
-    p.count = next - p.row0;
-    const int64_t tile = slot - first_slot(a, group, lo);
-    if (tile < 0 || tile * a.row_tile >= (int64_t)p.count * group) return false;
+  if (a.per) {
+    p.b = slot / a.per;
+    p.tile = slot - p.b * a.per;
+  } else {
+    p.b = last_at_most(c.batch + 1, slot, [&](int i) { return first_slot(a, group, i); });
+    const int64_t tile = slot - first_slot(a, group, p.b);
+    if (tile < 0 || tile > 0x7FFFFFFF) return false;
     p.tile = (int)tile;
-  } else {
-    const int per = (group + a.row_tile - 1 >> tile_shift(a));
-    p.b = p.row0 = slot / per;
-    p.tile = slot - p.b * per;
-    p.count = 1;
   }
+  if (!rows_of(c, p)) return false;
+  if ((int64_t)p.tile * a.row_tile >= (int64_t)p.count * group) return false;
   if (p.b == c.batch ? !a.fill_tail : !takes(a, group, p.count)) return false;
-  fill_place(a, group, p);
-  return true;
-}
-
-// The tile of a query row and head, the slot it had and its row in the tile;
-// false if no sequence of this pass has the row.
-__host__ __device__ inline bool place_of_row(const AttentionArgs& a, int group, int row, int head, Place& p,
-                                             int64_t& slot, int& index) {
-  const CacheArgs& c = a.c;
-  if (c.starts) {
-    int lo = 0, hi = c.batch;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (c.starts[mid] <= row) lo = mid; else hi = mid;
-    }
-    p.b = lo;
-    p.row0 = c.starts[lo];
-    const int next = c.starts[lo + 1];
-    if (p.row0 < 0 || row < p.row0 || row >= next || next > c.rows) return false;
-    p.count = next - p.row0;
-    slot = first_slot(a, group, lo);
-  } else {
-    p.b = p.row0 = row;
-    p.count = 1;
-    slot = (int64_t)row * ((group + a.row_tile - 1 >> tile_shift(a)));
-  }
-  if (!takes(a, group, p.count)) return false;
-  const int local = (row - p.row0) * group + head % group;
-  p.tile = local >> tile_shift(a);
-  index = local - p.tile * a.row_tile;
-  slot += p.tile;
   fill_place(a, group, p);
   return true;
 }
@@ -139,12 +138,7 @@ __host__ __device__ inline int64_t append_slots(const CacheArgs& c) {
 __host__ __device__ inline bool page_of_slot(const CacheArgs& c, int slot, PageWrite& w) {
   int b, row0, count, nth;
   if (c.starts) {
-    int lo = 0, hi = c.batch;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (c.starts[mid] / c.page + 2 * mid <= slot) lo = mid; else hi = mid;
-    }
-    b = lo;
+    b = last_at_most(c.batch, slot, [&](int i) { return (int64_t)c.starts[i] / c.page + 2 * i; });
     row0 = c.starts[b];
     const int next = c.starts[b + 1];
     if (row0 < 0 || next <= row0 || next > c.rows) return false;

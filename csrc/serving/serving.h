@@ -69,6 +69,7 @@ struct AttentionArgs {
   // of a pass, by plan_attention()
   int splits, chunk;      // workgroups of a context, and the tokens of one
   int row_tile;           // rows (token, head) of a workgroup
+  int per;                // tiles of a sequence, 0: as many as its rows need
   int few, many;          // takes the sequences with more than few, at most many rows
 };
 // Sequences with few rows and those with many take passes of their own.

@@ -371,7 +371,7 @@ def cache_attention(
     rows are its last tokens, whose keys and values the cache holds already.
     A row at position p sees the positions up to p, with ``window`` only the
     last ``window`` of them. ``q_heads`` is a multiple of the cache's heads.
-    ``scale`` is dim ** -0.5 unless given. ``max_seq_len``, the longest length
+    ``scale``, over 0, is dim ** -0.5 unless given. ``max_seq_len``, the longest length
     as far as the program knows it, only steers how work is split.
 
     Returns (out [T, q_heads, dim] in q's type, lse float32 [T, q_heads]), lse
@@ -394,8 +394,8 @@ def cache_attention(
         raise ValueError("more than 2^30 query rows")
     if scale is None:
         scale = dim**-0.5
-    elif not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, not {scale}")
+    elif not 0 < scale < math.inf:
+        raise ValueError(f"scale must be positive and finite, not {scale}")
     if window is not None and window < 1:
         raise ValueError(f"window must be at least 1, not {window}")
     if max_seq_len is None:

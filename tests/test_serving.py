@@ -258,6 +258,7 @@ def test_cache_attention_refuses(change, error, match):
         (torch.zeros(3, 4, 80, dtype=BF16), {}, ValueError, "head dimension 80"),
         (torch.zeros(3, 4, 64, dtype=BF16), dict(window=0), ValueError, "window"),
         (torch.zeros(3, 4, 64, dtype=BF16), dict(scale=float("inf")), ValueError, "scale"),
+        (torch.zeros(3, 4, 64, dtype=BF16), dict(scale=0.0), ValueError, "scale"),
         (torch.zeros(3, 4, 64, dtype=BF16), dict(out=torch.zeros(3, 4, 64)), TypeError, "out"),
         (torch.zeros(3, 4, 64, dtype=BF16), dict(out=torch.zeros(3, 64, 4, dtype=BF16).transpose(1, 2)), ValueError, "contiguous"),
         (torch.zeros(3, 4, 64, dtype=BF16, requires_grad=True), {}, ValueError, "no backward"),

@@ -349,6 +349,7 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
     float total = 0.f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) total += sums[w][t][r] * __builtin_amdgcn_exp2f(tops[w][t][r] - ref);
+    if (p.broken) total = __builtin_nanf("");
     const float f = __builtin_amdgcn_exp2f(top[t] - ref);
     if (t) __syncthreads();
 #pragma unroll
@@ -662,6 +663,7 @@ __global__ __launch_bounds__(kWaves * 64, DT <= 8 ? 2 : 1) void attention_rows_k
   for (int t = 0; t < QT; ++t) {
     sum[t] += __shfl_xor(sum[t], 16);
     sum[t] += __shfl_xor(sum[t], 32);
+    if (p.broken) sum[t] = __builtin_nanf("");
     const int i = mine + t * 16 + r;
     if (i >= p.rows) continue;
     if (p.splits == 1) {
@@ -786,7 +788,7 @@ hipError_t by_dim(const AttentionArgs& a, hipStream_t stream) {
 // Splits a pass's contexts; returns its floats of workspace.
 int64_t split(AttentionArgs& a, int64_t per_seq) {
   const int64_t slots = slot_count(a), work = slots * a.c.heads;
-  int64_t longest = a.longest > 0 ? a.longest : 1;
+  int64_t longest = a.longest < 1 ? 1 : a.longest > 1 << 30 ? 1 << 30 : a.longest;
   if (a.window && longest > a.window + kTile + per_seq) longest = a.window + kTile + per_seq;
   // Four rounds of workgroups on the card (2 fit a compute unit) even out their
   // lengths; more only add their beginnings and ends (64 contexts of 8-16k

@@ -51,127 +51,207 @@ class OnDevice {
 
 hipStream_t stream_of(uintptr_t s) { return reinterpret_cast<hipStream_t>(s); }
 
-W4Args w4_args(uintptr_t x, int64_t ldx, int m, int n, int k, int group, int dtype) {
+// The launches are called once an operator and step of a program, so they take
+// their whole numbers straight from the interpreter.
+class Numbers {
+ public:
+  Numbers(PyObject* const* args, Py_ssize_t count, Py_ssize_t wanted) : args_(args) {
+    if (count != wanted) throw std::invalid_argument("wrong number of arguments");
+  }
+  int64_t whole() {
+    PyObject* o = args_[at_++];
+    const int64_t v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) throw py::error_already_set();
+    return v;
+  }
+  int small() { return (int)whole(); }
+  template <typename T = void>
+  T* pointer() { return ptr<T>((uintptr_t)whole()); }
+  double real() {
+    const double v = PyFloat_AsDouble(args_[at_++]);
+    if (v == -1 && PyErr_Occurred()) throw py::error_already_set();
+    return v;
+  }
+
+ private:
+  PyObject* const* args_;
+  Py_ssize_t at_ = 0;
+};
+
+template <typename F>
+PyObject* guarded(F f) {
+  try {
+    return f();
+  } catch (py::error_already_set& e) {
+    e.restore();
+  } catch (const std::invalid_argument& e) {
+    PyErr_SetString(PyExc_TypeError, e.what());
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  }
+  return nullptr;
+}
+PyObject* none() { Py_RETURN_NONE; }
+
+W4Args w4_args(Numbers& n) {
   W4Args a{};
-  a.x = ptr<void>(x);
-  a.ldx = ldx;
-  a.m = m;
-  a.n = n;
-  a.k = k;
-  a.group = group;
-  a.dtype = dtype;
+  a.x = n.pointer();
+  a.ldx = n.whole();
+  a.m = n.small();
+  a.n = n.small();
+  a.k = n.small();
+  a.group = n.small();
+  a.dtype = n.small();
   return a;
 }
 
-int64_t w4_work(uintptr_t x, int64_t ldx, int m, int n, int k, int group, int dtype) {
-  return w4_workspace(w4_args(x, ldx, m, n, k, group, dtype));
+PyObject* w4_work(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  return guarded([&] {
+    Numbers n(args, count, 7);
+    return PyLong_FromLongLong(w4_workspace(w4_args(n)));
+  });
 }
 
-void w4_matmul(int device, uintptr_t stream, uintptr_t x, int64_t ldx, int m, int n, int k, int group, int dtype,
-               uintptr_t codes, uintptr_t scales, uintptr_t zeros, uintptr_t y, int64_t ldy, uintptr_t work) {
-  W4Args a = w4_args(x, ldx, m, n, k, group, dtype);
-  a.codes = ptr<uint8_t>(codes);
-  a.scales = ptr<void>(scales);
-  a.zeros = ptr<uint8_t>(zeros);
-  a.y = ptr<void>(y);
-  a.ldy = ldy;
-  a.work = ptr<void>(work);
-  OnDevice on(device);
-  OnDevice::check(launch_w4_matmul(a, stream_of(stream)), "w4_matmul");
+PyObject* w4_matmul(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  return guarded([&] {
+    Numbers n(args, count, 15);
+    W4Args a = w4_args(n);
+    a.codes = n.pointer<uint8_t>();
+    a.scales = n.pointer();
+    a.zeros = n.pointer<uint8_t>();
+    a.y = n.pointer();
+    a.ldy = n.whole();
+    a.work = n.pointer();
+    OnDevice on(n.small());
+    OnDevice::check(launch_w4_matmul(a, stream_of(n.whole())), "w4_matmul");
+    return none();
+  });
 }
 
-CacheArgs cache_args(const py::tuple& t) {
+CacheArgs cache_args(Numbers& n) {
   CacheArgs c{};
-  c.k = ptr<uint8_t>(t[0].cast<uintptr_t>());
-  c.v = ptr<uint8_t>(t[1].cast<uintptr_t>());
-  c.k_scale = ptr<float>(t[2].cast<uintptr_t>());
-  c.v_scale = ptr<float>(t[3].cast<uintptr_t>());
-  c.table = ptr<int32_t>(t[4].cast<uintptr_t>());
-  c.lens = ptr<int32_t>(t[5].cast<uintptr_t>());
-  c.starts = ptr<int32_t>(t[6].cast<uintptr_t>());
-  c.ldt = t[7].cast<int64_t>();
-  c.pages = t[8].cast<int>();
-  c.heads = t[9].cast<int>();
-  c.page = t[10].cast<int>();
-  c.dim = t[11].cast<int>();
-  c.batch = t[12].cast<int>();
-  c.blocks = t[13].cast<int>();
-  c.rows = t[14].cast<int>();
+  c.k = n.pointer<uint8_t>();
+  c.v = n.pointer<uint8_t>();
+  c.k_scale = n.pointer<float>();
+  c.v_scale = n.pointer<float>();
+  c.table = n.pointer<int32_t>();
+  c.lens = n.pointer<int32_t>();
+  c.starts = n.pointer<int32_t>();
+  c.ldt = n.whole();
+  c.pages = n.small();
+  c.heads = n.small();
+  c.page = n.small();
+  c.dim = n.small();
+  c.batch = n.small();
+  c.blocks = n.small();
+  c.rows = n.small();
   return c;
 }
 
-void cache_append(int device, uintptr_t stream, const py::tuple& cache, uintptr_t k, int64_t k_row, int64_t k_head,
-                  uintptr_t v, int64_t v_row, int64_t v_head, int dtype) {
-  AppendArgs a{};
-  a.c = cache_args(cache);
-  a.k_new = ptr<void>(k);
-  a.k_row = k_row;
-  a.k_head = k_head;
-  a.v_new = ptr<void>(v);
-  a.v_row = v_row;
-  a.v_head = v_head;
-  a.dtype = dtype;
-  OnDevice on(device);
-  OnDevice::check(launch_cache_append(a, stream_of(stream)), "cache_append");
+PyObject* cache_append(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  return guarded([&] {
+    Numbers n(args, count, 24);
+    AppendArgs a{};
+    a.c = cache_args(n);
+    a.k_new = n.pointer();
+    a.k_row = n.whole();
+    a.k_head = n.whole();
+    a.v_new = n.pointer();
+    a.v_row = n.whole();
+    a.v_head = n.whole();
+    a.dtype = n.small();
+    OnDevice on(n.small());
+    OnDevice::check(launch_cache_append(a, stream_of(n.whole())), "cache_append");
+    return none();
+  });
 }
 
-int64_t attention_floats(int rows, int batch, int heads, int q_heads, int dim, bool ragged, int window, int64_t longest) {
-  AttentionArgs a{};
-  static const int32_t some = 0;
-  a.c.rows = rows;
-  a.c.batch = batch;
-  a.c.heads = heads;
-  a.c.dim = dim;
-  a.c.starts = ragged ? &some : nullptr;  // only whether it is there counts
-  a.q_heads = q_heads;
-  a.window = window;
-  a.longest = longest;
-  return plan_attention(a).floats;
+PyObject* attention_floats(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  return guarded([&] {
+    Numbers n(args, count, 8);
+    AttentionArgs a{};
+    static const int32_t some = 0;
+    a.c.rows = n.small();
+    a.c.batch = n.small();
+    a.c.heads = n.small();
+    a.q_heads = n.small();
+    a.c.dim = n.small();
+    a.c.starts = n.whole() ? &some : nullptr;  // only whether it is there counts
+    a.window = n.small();
+    a.longest = n.whole();
+    return PyLong_FromLongLong(plan_attention(a).floats);
+  });
 }
 
-void cache_attention(int device, uintptr_t stream, const py::tuple& cache, uintptr_t q, int64_t q_row, int64_t q_head,
-                     uintptr_t out, int64_t o_row, int64_t o_head, uintptr_t lse, uintptr_t work, int q_heads,
-                     int window, int64_t longest, bool fill_tail, float scale, int dtype) {
-  AttentionArgs a{};
-  a.c = cache_args(cache);
-  a.q = ptr<void>(q);
-  a.q_row = q_row;
-  a.q_head = q_head;
-  a.out = ptr<void>(out);
-  a.o_row = o_row;
-  a.o_head = o_head;
-  a.lse = ptr<float>(lse);
-  a.work = ptr<float>(work);
-  a.q_heads = q_heads;
-  a.window = window;
-  a.longest = longest;
-  a.fill_tail = fill_tail;
-  a.scale = scale;
-  a.dtype = dtype;
-  OnDevice on(device);
-  OnDevice::check(launch_cache_attention(a, stream_of(stream)), "cache_attention");
+PyObject* cache_attention(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  return guarded([&] {
+    Numbers n(args, count, 31);
+    AttentionArgs a{};
+    a.c = cache_args(n);
+    a.q = n.pointer();
+    a.q_row = n.whole();
+    a.q_head = n.whole();
+    a.out = n.pointer();
+    a.o_row = n.whole();
+    a.o_head = n.whole();
+    a.lse = n.pointer<float>();
+    a.work = n.pointer<float>();
+    a.q_heads = n.small();
+    a.window = n.small();
+    a.longest = n.whole();
+    a.fill_tail = n.small();
+    a.scale = (float)n.real();
+    a.dtype = n.small();
+    OnDevice on(n.small());
+    OnDevice::check(launch_cache_attention(a, stream_of(n.whole())), "cache_attention");
+    return none();
+  });
 }
 
-void token_logprobs(int device, uintptr_t stream, uintptr_t logits, int64_t ld, uintptr_t targets, uintptr_t logprob,
-                    uintptr_t entropy, uintptr_t rank, uintptr_t top_ids, uintptr_t top_logprobs, uintptr_t work,
-                    int64_t rows, int vocab, int top, int dtype) {
-  LogprobArgs a{};
-  a.logits = ptr<void>(logits);
-  a.ld = ld;
-  a.targets = ptr<int64_t>(targets);
-  a.logprob = ptr<float>(logprob);
-  a.entropy = ptr<float>(entropy);
-  a.rank = ptr<int64_t>(rank);
-  a.top_ids = ptr<int64_t>(top_ids);
-  a.top_logprobs = ptr<float>(top_logprobs);
-  a.work = ptr<float>(work);
-  a.rows = rows;
-  a.vocab = vocab;
-  a.top = top;
-  a.dtype = dtype;
-  OnDevice on(device);
-  OnDevice::check(launch_token_logprobs(a, stream_of(stream)), "token_logprobs");
+PyObject* logprob_floats(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  return guarded([&] {
+    Numbers n(args, count, 3);
+    const int64_t rows = n.whole();
+    const int vocab = n.small();
+    return PyLong_FromLongLong(logprob_workspace(rows, vocab, n.small()));
+  });
 }
+
+PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  return guarded([&] {
+    Numbers n(args, count, 15);
+    LogprobArgs a{};
+    a.logits = n.pointer();
+    a.ld = n.whole();
+    a.targets = n.pointer<int64_t>();
+    a.logprob = n.pointer<float>();
+    a.entropy = n.pointer<float>();
+    a.rank = n.pointer<int64_t>();
+    a.top_ids = n.pointer<int64_t>();
+    a.top_logprobs = n.pointer<float>();
+    a.work = n.pointer<float>();
+    a.rows = n.whole();
+    a.vocab = n.small();
+    a.top = n.small();
+    a.dtype = n.small();
+    OnDevice on(n.small());
+    OnDevice::check(launch_token_logprobs(a, stream_of(n.whole())), "token_logprobs");
+    return none();
+  });
+}
+
+#define FAST(name, f) {name, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
+PyMethodDef launches[] = {
+    FAST("w4_workspace", w4_work),
+    FAST("w4_matmul", w4_matmul),
+    FAST("cache_append", cache_append),
+    FAST("attention_workspace", attention_floats),
+    FAST("cache_attention", cache_attention),
+    FAST("logprob_workspace", logprob_floats),
+    FAST("token_logprobs", token_logprobs),
+    {nullptr, nullptr, 0, nullptr},
+};
+#undef FAST
 
 // What the kernels derive from host copies of lengths, starts and tables, for
 // checks on the host: (row, head, slot, split, lo, hi) of every row that a
@@ -257,18 +337,12 @@ py::dict step(int device, int iters, uint32_t seed, double oracle_offset) {
 
 PYBIND11_MODULE(_serving, m) {
   m.doc() = "gpud_amd CDNA4 serving-step operators (4-bit products, 8-bit cache, token log probabilities)";
-  m.def("w4_workspace", &w4_work);
-  m.def("w4_matmul", &w4_matmul);
-  m.def("cache_append", &cache_append);
-  m.def("attention_workspace", &attention_floats);
-  m.def("cache_attention", &cache_attention);
-  m.def("logprob_workspace", &logprob_workspace);
+  if (PyModule_AddFunctions(m.ptr(), launches) != 0) throw py::error_already_set();
   m.def("serving_step", &step, py::arg("device") = 0, py::arg("iters") = 20, py::arg("seed") = 1,
         py::arg("oracle_offset") = 0.0,
         "One token step of a synthetic served model, checked against host oracles; returns rates + verification");
   m.def("attention_places", &attention_places);
   m.def("append_places", &append_places);
-  m.def("token_logprobs", &token_logprobs);
   m.attr("MAX_COLUMNS") = kMaxColumns;
   m.attr("MAX_TOP") = kMaxTop;
   m.attr("MAX_VOCAB") = kMaxVocab;

@@ -232,8 +232,14 @@ __global__ __launch_bounds__(256, 4) void spans_kernel(LogprobArgs a) {
 
 // Lists of (order, place) in LDS, one list a wave; a key is larger where the
 // value is, and among equal values where the place is lower. A list holds the
-// spans, then at most 64 members of each of `top` parts.
-inline int list_size(int spans, int top) { return top == 0 ? 0 : spans > 64 * top ? spans : 64 * top; }
+// groups, or where they are many the spans, then at most 64 members of each of
+// `top` parts.
+constexpr int kDirect = 1024;
+inline int list_size(const Layout& lay, int top) {
+  const int64_t groups = (int64_t)lay.spans * lay.groups;
+  const int first = groups <= kDirect ? (int)groups : lay.spans;
+  return top == 0 ? 0 : first > 64 * top ? first : 64 * top;
+}
 
 __device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t place) {
   return (uint64_t)order << 32 | (uint32_t)~place;
@@ -253,7 +259,7 @@ __device__ void select_top(uint64_t* list, int n, int want, uint64_t* out, int l
     uint64_t mine = 0;
     for (int i = lane; i < n; i += 64) mine = list[i] > mine ? list[i] : mine;
     int place = 0;
-#pragma unroll
+#pragma unroll 4
     for (int j = 0; j < 64; ++j) place += of_lane(mine, j) > mine;
     uint64_t low = of_lane(mine, __ffsll((unsigned long long)__ballot(place == want - 1)) - 1);
     auto keep = [&] {
@@ -287,7 +293,7 @@ __device__ void select_top(uint64_t* list, int n, int want, uint64_t* out, int l
   for (int i = lane; i < n; i += 64) {
     const uint64_t key = list[i];
     int place = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (int j = 0; j < n; ++j) place += list[j] > key;
     if (place < want) out[place] = key;
   }
@@ -302,6 +308,16 @@ __global__ __launch_bounds__(64) void rows_kernel(LogprobArgs a) {
   const T* x = (const T*)a.logits + row * a.ld;
   const int64_t t = a.targets[row];
   const bool known = t >= 0 && t < a.vocab;
+
+  extern __shared__ uint64_t list[];  // list_size()
+  __shared__ uint64_t out[3][kMaxTop];
+  // groups of 64 where they are few enough to go through at once, else spans
+  const bool direct = (int64_t)lay.spans * lay.groups <= kDirect;
+  int n = direct ? lay.spans * lay.groups : lay.spans;
+  if (a.top) {
+    const float* from = direct ? lay.group(a.work, row, 0) : lay.tops(a.work, row);
+    for (int i = lane; i < n; i += 64) list[i] = key_of(order_of(from[i]), i);
+  }
 
   // the spans' sums against one reference, each lane's in the spans' order
   const float* stats = lay.stats(a.work, row, 0);
@@ -336,51 +352,49 @@ __global__ __launch_bounds__(64) void rows_kernel(LogprobArgs a) {
   }
   if (a.top == 0) return;
 
-  extern __shared__ uint64_t list[];  // list_size()
-  __shared__ uint64_t out[3][kMaxTop];
   const int want = a.top;
   const int shift = (int)(((uintptr_t)x / sizeof(T)) % S::kVec);
-  const float* tops = lay.tops(a.work, row);
-
-  // spans, then groups of 64, then logits
-  int n = lay.spans;
-  for (int i = lane; i < n; i += 64) list[i] = key_of(order_of(tops[i]), i);
-  __syncthreads();
-  int got = n < want ? n : want;
-  select_top(list, n, got, out[0], lane);
-  __syncthreads();
+  int got = 0;
+  // one body for all levels: a lone wave waits for every line of new code
 #pragma unroll 1
-  for (int level = 1; level <= 2; ++level) {
-    // members of the last level's parts; those under its least are left out
-    const int parts = got;
-    const int size = level == 1 ? S::kGroups : 64;
-    const uint32_t least = parts == want ? (uint32_t)(out[level - 1][parts - 1] >> 32) : 0u;
-    n = 0;
-    constexpr int kBatch = 8;
-    for (int first = 0; first < parts; first += kBatch) {
-      uint32_t order[kBatch], place[kBatch];
-      bool in[kBatch];
+  for (int level = direct ? 1 : 0, first_level = level; level <= 2; ++level) {
+    if (level > first_level) {
+      // members of the last level's parts; those under its least are left out
+      const int parts = got;
+      const int size = level == 1 ? S::kGroups : 64;
+      const uint32_t least = parts == want ? (uint32_t)(out[level - 1][parts - 1] >> 32) : 0u;
+      n = 0;
+      constexpr int kBatch = 8;
+#pragma unroll 1
+      for (int first = 0; first < parts; first += kBatch) {
+        uint32_t place[kBatch];
+        float value[kBatch];
+        bool in[kBatch];
 #pragma unroll
-      for (int q = 0; q < kBatch; ++q) {
-        const uint32_t part = ~(uint32_t)out[level - 1][first + q < parts ? first + q : parts - 1];
-        place[q] = part * size + lane;
-        in[q] = first + q < parts && lane < size;
-        float v = 0.f;
-        if (level == 1) {
-          if (in[q]) v = lay.group(a.work, row, 0)[place[q]];
-        } else {
-          place[q] -= shift;
-          in[q] = in[q] && place[q] < (uint32_t)a.vocab;
-          if (in[q]) v = (float)x[place[q]];
+        for (int q = 0; q < kBatch; ++q) {  // loads without a branch, so that none waits for another
+          const uint32_t part = ~(uint32_t)out[level - 1][first + q < parts ? first + q : parts - 1];
+          place[q] = part * size + lane - (level == 1 ? 0 : shift);
+          in[q] = first + q < parts && lane < size && (level == 1 || place[q] < (uint32_t)a.vocab);
         }
-        order[q] = order_of(v);
-      }
+        if (level == 1) {
+          const float* from = lay.group(a.work, row, 0);
 #pragma unroll
-      for (int q = 0; q < kBatch; ++q) {
-        const bool kept = in[q] && order[q] >= least;
-        const uint64_t mask = __ballot(kept);
-        if (kept) list[n + __popcll(mask & ((1ull << lane) - 1))] = key_of(order[q], place[q]);
-        n += __popcll(mask);
+          for (int q = 0; q < kBatch; ++q) value[q] = from[in[q] ? place[q] : 0];
+        } else {
+          T raw[kBatch];
+#pragma unroll
+          for (int q = 0; q < kBatch; ++q) raw[q] = x[in[q] ? place[q] : 0];
+#pragma unroll
+          for (int q = 0; q < kBatch; ++q) value[q] = (float)raw[q];
+        }
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q) {
+          const uint32_t order = order_of(value[q]);
+          const bool kept = in[q] && order >= least;
+          const uint64_t mask = __ballot(kept);
+          if (kept) list[n + __popcll(mask & ((1ull << lane) - 1))] = key_of(order, place[q]);
+          n += __popcll(mask);
+        }
       }
     }
     __syncthreads();
@@ -401,7 +415,7 @@ hipError_t launch(const LogprobArgs& a, hipStream_t stream) {
   const dim3 grid((lay.spans + 3) / 4, a.rows < 65535 ? (int)a.rows : 65535);
   spans_kernel<T><<<grid, 256, 0, stream>>>(a);
   if (hipError_t e = hipGetLastError()) return e;
-  const size_t lds = sizeof(uint64_t) * list_size(lay.spans, a.top);
+  const size_t lds = sizeof(uint64_t) * list_size(lay, a.top);
   rows_kernel<T><<<dim3((unsigned)a.rows), 64, lds, stream>>>(a);
   return hipGetLastError();
 }

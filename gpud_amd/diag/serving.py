@@ -44,8 +44,11 @@ __all__ = [
 ]
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_CODES = (torch.float8_e4m3fn, torch.uint8)
+_HALVES = {torch.bfloat16: 0, torch.float16: 1}
+F8 = torch.float8_e4m3fn
+_CODES = (F8, torch.uint8)
 _INT_MAX = 2**31 - 1
+_MOST = 2**30
 
 GROUPS = (32, 64, 128)
 MAX_COLUMNS = _serving.MAX_COLUMNS
@@ -54,8 +57,7 @@ MAX_VOCAB = _serving.MAX_VOCAB
 MAX_HEAD_DIM = 256
 
 
-def _stream(device: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
+_stream = torch._C._cuda_getCurrentRawStream  # of a device number
 
 
 def _fits(t, device: int, dtype, shape) -> bool:
@@ -68,6 +70,13 @@ def _fits(t, device: int, dtype, shape) -> bool:
         and t.is_contiguous()
         and not t.requires_grad
     )
+
+
+def _primary(name: str, t, dim: int, dtypes) -> int:
+    """The native number of the type of a call's first tensor, which has to be in `dtypes`."""
+    if type(t) is not torch.Tensor or t.dtype not in dtypes or t.dim() != dim or t.requires_grad:
+        _check_input(name, t, None, tuple(dtypes), dim)
+    return dtypes[t.dtype]
 
 
 def _check_input(name: str, t: torch.Tensor, device: Optional[torch.device], dtypes, dim: int) -> None:
@@ -175,8 +184,7 @@ def w4_matmul(
     M up to 64; larger M are taken 64 rows at a time, K up to ``MAX_COLUMNS``.
     Sums are fp32, rounded once to x's type. ``x`` has to be finite, and under 1e37 in magnitude.
     """
-    _check_input("x", x, None, (torch.bfloat16, torch.float16), 2)
-    device = x.device
+    dtype = _primary("x", x, 2, _HALVES)
     m, k = x.shape
     n = int(out_features)
     if group_size not in GROUPS:
@@ -184,7 +192,7 @@ def w4_matmul(
     if k < 1 or n < 1 or k > MAX_COLUMNS or n > _INT_MAX // 2 or m > 65535 * 16:
         raise ValueError(f"no product of {m} rows with weights [{n}, {k}]")
     tiles, groups = -(-n // 16), -(-k // group_size)
-    at = x.get_device()
+    at, device = x.get_device(), x.device
     if not _fits(codes, at, torch.uint8, (tiles, -(-k // 128), 64, 16)):
         _check_input("codes", codes, device, (torch.uint8,), 4)
         _check_shape("codes", codes, (tiles, -(-k // 128), 64, 16))
@@ -194,11 +202,11 @@ def w4_matmul(
     if zeros is not None and not _fits(zeros, at, torch.uint8, (tiles, groups, 16)):
         _check_input("zeros", zeros, device, (torch.uint8,), 3)
         _check_shape("zeros", zeros, (tiles, groups, 16))
-    if codes.data_ptr() % 16 or scales.data_ptr() % 8:
-        raise ValueError("codes and scales must be aligned to 16 and 8 bytes")
+    if codes.data_ptr() % 16 or scales.data_ptr() % 8 or (zeros is not None and zeros.data_ptr() % 4):
+        raise ValueError("codes, scales and zeros must be aligned to 16, 8 and 4 bytes")
     if out is None:
         _check_gpu(device)
-        out = torch.empty(m, n, dtype=x.dtype, device=device)
+        out = x.new_empty((m, n))
     else:
         _check_input("out", out, device, (x.dtype,), 2)
         if tuple(out.shape) != (m, n) or (out.stride(1) != 1 and n > 1):
@@ -209,12 +217,12 @@ def w4_matmul(
     if x.stride(1) != 1 and k > 1:
         x = x.contiguous()
     if m:
-        args = (x.data_ptr(), x.stride(0), m, n, k, group_size, _DTYPES[x.dtype])
+        args = (x.data_ptr(), x.stride(0), m, n, k, group_size, dtype)
         size = _serving.w4_workspace(*args)
         work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         _serving.w4_matmul(
-            device.index, _stream(device), *args, codes.data_ptr(), scales.data_ptr(),
-            0 if zeros is None else zeros.data_ptr(), out.data_ptr(), out.stride(0), work.data_ptr() if size else 0,
+            *args, codes.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(),
+            out.data_ptr(), out.stride(0), work.data_ptr() if size else 0, at, _stream(at),
         )
     return out
 
@@ -261,29 +269,32 @@ def _check_cache_sizes(pages: int, heads: int, page: int, dim: int) -> None:
         raise ValueError(f"head dimension must be a multiple of 16 up to {MAX_HEAD_DIM}, not {dim}")
 
 
-def _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start, device, rows):
-    _check_input("k_cache", k_cache, device, _CODES, 4)
+def _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start, device, at, rows):
+    if type(k_cache) is not torch.Tensor or k_cache.dim() != 4 or not _fits(k_cache, at, F8, k_cache.shape):
+        _check_input("k_cache", k_cache, device, _CODES, 4)
+        if not k_cache.is_contiguous():
+            raise ValueError("k_cache must be contiguous")
     pages, heads, page, dim = k_cache.shape
     _check_cache_sizes(pages, heads, page, dim)
-    if not k_cache.is_contiguous():
-        raise ValueError("k_cache must be contiguous")
-    at = k_cache.get_device()
     if not _fits(v_cache, at, k_cache.dtype, (pages, heads, dim, page)):
         _check_input("v_cache", v_cache, device, _CODES, 4)
         _check_shape("v_cache", v_cache, (pages, heads, dim, page))
-    for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if not _fits(scale, at, torch.float32, (pages, heads)):
-            _check_input(name, scale, device, (torch.float32,), 2)
-            _check_shape(name, scale, (pages, heads))
-    _check_input("block_table", block_table, device, (torch.int32,), 2)
+    if not _fits(k_scale, at, torch.float32, (pages, heads)):
+        _check_input("k_scale", k_scale, device, (torch.float32,), 2)
+        _check_shape("k_scale", k_scale, (pages, heads))
+    if not _fits(v_scale, at, torch.float32, (pages, heads)):
+        _check_input("v_scale", v_scale, device, (torch.float32,), 2)
+        _check_shape("v_scale", v_scale, (pages, heads))
+    if type(block_table) is not torch.Tensor or block_table.dim() != 2 or not _fits(block_table, at, torch.int32, block_table.shape):
+        _check_input("block_table", block_table, device, (torch.int32,), 2)
+        if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+            raise ValueError("rows of block_table must be dense")
     batch, blocks = block_table.shape
-    if blocks > 1 and block_table.stride(1) != 1:
-        raise ValueError("rows of block_table must be dense")
     if not _fits(seq_lens, at, torch.int32, (batch,)):
         _check_input("seq_lens", seq_lens, device, (torch.int32,), 1)
         _check_shape("seq_lens", seq_lens, (batch,))
-    if blocks * page > _INT_MAX:
-        raise ValueError("block_table covers more than 2^31 - 1 positions")
+    if blocks * page > _MOST or batch * heads > _INT_MAX // 64:
+        raise ValueError("block_table covers more than 2^30 positions, or too many sequences and heads")
     starts = 0
     if query_start is None:
         if rows != batch:
@@ -328,15 +339,15 @@ def cache_append(
     out of range, or whose position is negative, are left out. A page that gets
     tokens may belong to one sequence only.
     """
-    _check_input("k", k, None, (torch.bfloat16, torch.float16), 3)
-    device = k.device
+    dtype = _primary("k", k, 3, _HALVES)
+    device, at = k.device, k.get_device()
     _check_input("v", v, device, (k.dtype,), 3)
     rows = k.shape[0]
-    cache = _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start, device, rows)
+    cache = _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start, device, at, rows)
     heads, dim, batch = cache[9], cache[11], cache[12]
-    if tuple(k.shape) != (rows, heads, dim) or tuple(v.shape) != (rows, heads, dim):
+    if k.shape != (rows, heads, dim) or v.shape != (rows, heads, dim):
         raise ValueError(f"k and v must be [T, {heads}, {dim}], not {tuple(k.shape)} and {tuple(v.shape)}")
-    if rows * heads > _INT_MAX // 2:
+    if rows * heads > _MOST:
         raise ValueError("more than 2^30 new keys")
     _check_gpu(device)
     if k.stride(2) != 1:
@@ -345,8 +356,8 @@ def cache_append(
         v = v.contiguous()
     if rows and batch:
         _serving.cache_append(
-            device.index, _stream(device), cache, k.data_ptr(), k.stride(0), k.stride(1),
-            v.data_ptr(), v.stride(0), v.stride(1), _DTYPES[k.dtype],
+            *cache, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+            dtype, at, _stream(at),
         )
 
 
@@ -375,22 +386,23 @@ def cache_attention(
     as far as the program knows it, only steers how work is split.
 
     Returns (out [T, q_heads, dim] in q's type, lse float32 [T, q_heads]), lse
-    the logarithm of the sum of the exponentials of a row's scores. A row that
+    the logarithm of the sum of the exponentials of a row's scores. The scales
+    of pages that are read have to be positive and finite. A row that
     sees nothing gets 0 and -inf. A sequence whose pages are out of range, or
     that is longer than its row of ``block_table``, gets NaN. Rows behind the
     last sequence are left as they were in ``out`` if that is given, and else
     0; their lse is -inf.
     """
-    _check_input("q", q, None, (torch.bfloat16, torch.float16), 3)
-    device = q.device
+    dtype = _primary("q", q, 3, _HALVES)
+    device, at = q.device, q.get_device()
     rows, q_heads, dim = q.shape
-    cache = _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start, device, rows)
+    cache = _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start, device, at, rows)
     heads, batch = cache[9], cache[12]
     if dim != cache[11]:
         raise ValueError(f"q has head dimension {dim}, the cache {cache[11]}")
     if q_heads < 1 or q_heads % heads or q_heads > 65535:
         raise ValueError(f"{q_heads} query heads do not share {heads} cached ones evenly")
-    if rows * q_heads > _INT_MAX // 2:
+    if rows * q_heads > _MOST or batch * q_heads > _MOST:
         raise ValueError("more than 2^30 query rows")
     if scale is None:
         scale = dim**-0.5
@@ -398,8 +410,8 @@ def cache_attention(
         raise ValueError(f"scale must be positive and finite, not {scale}")
     if window is not None and window < 1:
         raise ValueError(f"window must be at least 1, not {window}")
-    if max_seq_len is None:
-        max_seq_len = cache[13] * cache[10]
+    room = cache[13] * cache[10]
+    max_seq_len = room if max_seq_len is None else min(max_seq_len, room)
     fill = out is None
     if not fill:
         _check_input("out", out, device, (q.dtype,), 3)
@@ -408,10 +420,12 @@ def cache_attention(
             raise ValueError("out must be aligned to 8 bytes")
     _check_gpu(device)
     # 16-byte loads of the queries
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+    row, head, one = q.stride()
+    if one != 1 or row % 8 or head % 8 or q.data_ptr() % 16:
+        row, head = q_heads * dim, dim
         q = q.clone(memory_format=torch.contiguous_format)
     if fill:
-        out = torch.empty(rows, q_heads, dim, dtype=q.dtype, device=device)
+        out = q.new_empty((rows, q_heads, dim))
     lse = torch.empty(rows, q_heads, dtype=torch.float32, device=device)
     if not rows:
         return out, lse
@@ -420,15 +434,15 @@ def cache_attention(
             out.zero_()
         lse.fill_(-math.inf)
         return out, lse
-    window = min(window or 0, _INT_MAX // 2)
+    window = min(window, _MOST) if window else 0
     floats = _serving.attention_workspace(
         rows, batch, heads, q_heads, dim, query_start is not None, window, max_seq_len
     )
     work = torch.empty(floats, dtype=torch.float32, device=device) if floats else None
     _serving.cache_attention(
-        device.index, _stream(device), cache, q.data_ptr(), q.stride(0), q.stride(1),
-        out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), work.data_ptr() if floats else 0,
-        q_heads, window, max_seq_len, fill, scale, _DTYPES[q.dtype],
+        *cache, q.data_ptr(), row, head, out.data_ptr(), q_heads * dim, dim, lse.data_ptr(),
+        work.data_ptr() if floats else 0,
+        q_heads, window, max_seq_len, fill, scale, dtype, at, _stream(at),
     )
     return out, lse
 
@@ -458,12 +472,14 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
     row with NaN or +inf has NaN as its log probability and entropy; NaN comes
     first among its alternatives.
     """
-    _check_input("logits", logits, None, _DTYPES, 2)
-    device = logits.device
+    dtype = _primary("logits", logits, 2, _DTYPES)
+    device, at = logits.device, logits.get_device()
     rows, vocab = logits.shape
-    _check_input("targets", targets, device, (torch.int64,), 1)
-    if targets.shape[0] != rows:
-        raise ValueError(f"{targets.shape[0]} targets for {rows} rows")
+    if not _fits(targets, at, torch.int64, (rows,)):
+        _check_input("targets", targets, device, (torch.int64,), 1)
+        if targets.shape[0] != rows:
+            raise ValueError(f"{targets.shape[0]} targets for {rows} rows")
+        targets = targets.contiguous()
     if vocab < 1 or vocab > MAX_VOCAB:
         raise ValueError(f"vocabulary must have 1..{MAX_VOCAB} tokens, not {vocab}")
     if top_k < 0 or top_k > min(MAX_TOP, vocab):
@@ -473,21 +489,17 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
     _check_gpu(device)
     if logits.stride(1) != 1 and vocab > 1:
         logits = logits.contiguous()
-    targets = targets.contiguous()
     logprob = torch.empty(rows, dtype=torch.float32, device=device)
-    entropy = torch.empty_like(logprob)
-    rank = torch.empty(rows, dtype=torch.int64, device=device)
+    entropy = logprob.new_empty(rows)
+    rank = targets.new_empty(rows)
     top_ids = top_logprobs = None
     if top_k:
-        top_ids = torch.empty(rows, top_k, dtype=torch.int64, device=device)
-        top_logprobs = torch.empty(rows, top_k, dtype=torch.float32, device=device)
+        top_ids, top_logprobs = rank.new_empty((rows, top_k)), logprob.new_empty((rows, top_k))
     if rows:
-        dtype = _DTYPES[logits.dtype]
-        work = torch.empty(_serving.logprob_workspace(rows, vocab, dtype), dtype=torch.float32, device=device)
+        work = logprob.new_empty(_serving.logprob_workspace(rows, vocab, dtype))
         _serving.token_logprobs(
-            device.index, _stream(device), logits.data_ptr(), logits.stride(0), targets.data_ptr(),
-            logprob.data_ptr(), entropy.data_ptr(), rank.data_ptr(),
-            top_ids.data_ptr() if top_k else 0, top_logprobs.data_ptr() if top_k else 0,
-            work.data_ptr(), rows, vocab, top_k, dtype,
+            logits.data_ptr(), logits.stride(0), targets.data_ptr(), logprob.data_ptr(), entropy.data_ptr(),
+            rank.data_ptr(), top_ids.data_ptr() if top_k else 0, top_logprobs.data_ptr() if top_k else 0,
+            work.data_ptr(), rows, vocab, top_k, dtype, at, _stream(at),
         )
     return TokenLogprobs(logprob, entropy, rank, top_ids, top_logprobs)

@@ -188,6 +188,7 @@ def w4_args(**change):
         (dict(codes=torch.zeros(2, 2, 64, 32, dtype=torch.uint8)[..., ::2]), ValueError, "contiguous"),
         (dict(zeros=torch.zeros(2, 2, 16)), TypeError, "zeros"),
         (dict(zeros=torch.zeros(2, 1, 16, dtype=torch.uint8)), ValueError, "zeros has shape"),
+        (dict(zeros=torch.zeros(65, dtype=torch.uint8)[1:].view(2, 2, 16)), ValueError, "aligned"),
         (dict(out=torch.zeros(3, 20)), TypeError, "out"),
         (dict(out=torch.zeros(3, 21, dtype=BF16)), ValueError, "out must be"),
         (dict(out=torch.zeros(20, dtype=BF16).expand(3, 20)), ValueError, "overlap"),
@@ -225,6 +226,7 @@ BAD_CACHE = [
     (dict(seq_lens=torch.ones(2, dtype=torch.int32)), ValueError, "seq_lens has shape"),
     (dict(seq_lens=torch.ones(3, dtype=torch.long)), TypeError, "seq_lens"),
     (dict(query_start=torch.zeros(3, dtype=torch.int32)), ValueError, "query_start has shape"),
+    (dict(block_table=torch.zeros(3, 2**26 + 1, dtype=torch.int32)), ValueError, "2\\^30 positions"),
     (dict(block_table=torch.zeros(2, 4, dtype=torch.int32), seq_lens=torch.ones(2, dtype=torch.int32)), ValueError, "query_start"),
 ]
 

@@ -432,6 +432,55 @@ def test_attention_bad_pages_and_lengths(serving):
     assert not bool(torch.isnan(out).any()) and bool((out[2] == 0).all()) and bool((lse[2] == -INF).all())
 
 
+@pytest.mark.parametrize("count", [1, 5, 40, 100])
+def test_attention_longer_than_its_table_is_nan(serving, count):
+    """Every row of such a sequence, also with no table at all; its neighbours are not touched."""
+    cache, _, _ = filled(serving, [120, 120], 2, 64, 16)
+    q = torch.randn(2 * count, 8, 64, generator=gen(1), device="cuda").to(BF16)
+    starts = [0, count, 2 * count]
+    out, lse = serving.cache_attention(q, *cache.tensors, cache.table, ints([8 * 16 + 1, 120]), ints(starts))
+    assert bool(torch.isnan(out[:count]).all()) and bool(torch.isnan(lse[:count]).all())
+    check_attention(cache, q, [120, 120], starts, (out, lse), skip=(0,))
+    for blocks in (0, 1):
+        out, lse = serving.cache_attention(q, *cache.tensors, cache.table[:, :blocks], ints([120, 0]), ints(starts))
+        assert bool(torch.isnan(out[:count]).all()) and bool(torch.isnan(lse[:count]).all())
+        assert bool((out[count:] == 0).all()) and bool((lse[count:] == -INF).all())
+
+
+@pytest.mark.parametrize("window", [None, 70])
+def test_attention_mixed_batches_of_long_chunks(serving, window):
+    """Sequences of many rows and of few take passes of their own; rows behind them too."""
+    lens, counts = [600, 90, 1, 0, 333, 70, 2000], [300, 1, 1, 0, 7, 70, 130]
+    for dim, group in ((128, 4), (64, 8), (208, 3)):
+        cache, _, _ = filled(serving, lens, 2, dim, 32, seed=dim)
+        starts = starts_of(counts)
+        q = torch.randn(starts[-1] + 9, 2 * group, dim, generator=gen(2), device="cuda").to(BF16)
+        for longest in (None, 1):
+            got = serving.cache_attention(q, *cache.tensors, cache.table, ints(lens), ints(starts), window=window, max_seq_len=longest)
+            check_attention(cache, q, lens, starts, got, window=window)
+            assert bool((got[0][starts[-1]:] == 0).all()) and bool((got[1][starts[-1]:] == -INF).all())
+        mine = torch.full_like(q, 3.0)
+        serving.cache_attention(q, *cache.tensors, cache.table, ints(lens), ints(starts), window=window, out=mine)
+        check_attention(cache, q, lens, starts, (mine, got[1]), window=window)
+        assert bool((mine[starts[-1]:] == 3).all())
+
+
+def test_attention_masked_nan_in_long_chunks(serving):
+    lens, counts = [400], [200]
+    cache = Cache(serving, lens, 1, 128, 64)
+    k, v = (torch.randn(400, 1, 128, generator=gen(i), device="cuda").to(BF16) for i in (1, 2))
+    v[300, 0, 77] = NAN
+    serving.cache_append(k, v, *cache.tensors, cache.table, ints(lens), ints([0, 400]))
+    q = torch.randn(200, 4, 128, generator=gen(3), device="cuda").to(BF16)
+    for window in (None, 30):
+        out, lse = serving.cache_attention(q, *cache.tensors, cache.table, ints(lens), ints([0, 200]), window=window)
+        pos = torch.arange(200, 400, device="cuda")
+        sees = (pos >= 300) & ((pos < 330) if window else True)
+        bad = torch.isnan(out)
+        assert torch.equal(bad[..., 77], sees[:, None].expand(-1, 4)) and int(bad.sum()) == int(sees.sum()) * 4
+        assert not bool(torch.isnan(lse).any())
+
+
 def test_attention_offsets_past_32_bits(serving):
     """Pages whose bytes lie beyond 2^31 and 2^32."""
     heads, dim, page = 8, 128, 64

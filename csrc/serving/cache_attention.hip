@@ -97,6 +97,14 @@ __device__ __forceinline__ u32x4 load16(const uint8_t* p) {
   return *reinterpret_cast<const u32x4*>(p);
 }
 
+// The same number, but one that the compiler does not know to be: what depends
+// on it is worked out where it stands, not ahead of a loop, where it would take
+// more scalar registers than there are.
+__device__ __forceinline__ int anew(int v) {
+  asm volatile("" : "+s"(v));
+  return v;
+}
+
 constexpr int waves_of(int dt, int qt) { return dt * qt <= 4 ? 3 : dt * qt <= 8 ? 2 : 1; }
 
 template <typename T, int DT, int QT, bool kWhole>
@@ -161,6 +169,7 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
   u32x4 kr[4][KB], vr[DT];
   float ks, vs;
   auto load_keys = [&](int base, const Pages& at) {
+    const int dim = kWhole ? DT * 16 : anew(c.dim);
     const int pid = __shfl(at.pid, (r >> 2) << 4);
     const int tok = ((base + ((r >> 2) << 4)) & (page - 1)) + (r & 3);
     const uint8_t* from = c.k + (((int64_t)pid * c.heads + h) * page + tok) * dim + g * 16;
@@ -177,10 +186,11 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
     vs = c.v_scale[ph];
   };
   auto load_values = [&](int base, const Pages& at) {
+    const int dim = kWhole ? DT * 16 : anew(c.dim), page = anew(c.page);
     const uint8_t* from = c.v + (((int64_t)at.pid * c.heads + h) * dim + r) * page + ((base + g * 16) & (page - 1));
 #pragma unroll
     for (int d = 0; d < DT; ++d)
-      vr[d] = load16<QT>(from + (kWhole || d * 16 < dim ? d : 0) * 16 * page);
+      vr[d] = load16<QT>(from + (kWhole ? d : min(d, (dim >> 4) - 1)) * 16 * page);
   };
 
   // Takes the wave's tiles. A tile at the edge of what the rows see may hold

@@ -338,7 +338,7 @@ def test_attention_single_tokens(serving, heads, group, dim, page, dtype):
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("window", [None, 1, 50, 64, 400])
-@pytest.mark.parametrize("heads,group,dim,page", [(2, 4, 128, 64), (1, 1, 64, 16), (2, 8, 64, 32), (1, 7, 128, 16), (1, 32, 256, 16)])
+@pytest.mark.parametrize("heads,group,dim,page", [(2, 4, 128, 64), (1, 1, 64, 16), (2, 8, 64, 32), (1, 7, 128, 16), (1, 32, 256, 16), (2, 3, 208, 16), (1, 16, 80, 64), (3, 1, 48, 128)])
 def test_attention_chunks(serving, heads, group, dim, page, window, dtype):
     lens = [700, 1, 33, 0, 64, 500, 129]
     counts = [5, 1, 33, 0, 20, 150, 1]

@@ -62,12 +62,11 @@ __device__ __forceinline__ void unpack(u32x4 v, float* f, const float*) {
 // Larger of a lane's and another's; NaN gives way.
 __device__ __forceinline__ float max_xor(float v, int mask) { return fmaxf(v, __shfl_xor(v, mask)); }
 
-// Largest of kLanes neighbours (8 or 16), in all of them; NaN gives way. A step
-// is one instruction, whose second operand comes from the other lane.
+// Largest of kLanes neighbours (8 or 16), in all of them; a NaN stays.
 template <int kControl>
 __device__ __forceinline__ float max_dpp(float v) {
   const int other = __builtin_amdgcn_update_dpp(0, bits_as<int>(v), kControl, 0xF, 0xF, true);
-  return fmaxf(v, bits_as<float>(other));
+  return __builtin_elementwise_maximum(v, bits_as<float>(other));
 }
 template <int kLanes>
 __device__ __forceinline__ float group_max(float v) {
@@ -89,7 +88,7 @@ __device__ __forceinline__ float value_of(uint32_t order) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(256, 4) void spans_kernel(LogprobArgs a) {
+__global__ __launch_bounds__(256, 5) void spans_kernel(LogprobArgs a) {
   using S = Shape<T>;
   constexpr int V = S::kVec;
   const Layout lay(a.vocab, S::kSpan);
@@ -132,22 +131,19 @@ __global__ __launch_bounds__(256, 4) void spans_kernel(LogprobArgs a) {
     };
     float best[kUnits];  // of the lane's group of 64 values
     float m = -kInf;
-    bool nan = false;
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       float f[V];
       unpack(raw[u], f, (const T*)nullptr);
       float b = f[0];
 #pragma unroll
-      for (int i = 1; i < V; ++i) b = __builtin_elementwise_maximum(b, f[i]);  // keeps a NaN
-      nan |= b != b;
+      for (int i = 1; i < V; ++i) b = __builtin_elementwise_maximum(b, f[i]);  // a NaN stays
       best[u] = group_max<S::kLanes>(b);
-      m = fmaxf(m, best[u]);
+      m = __builtin_elementwise_maximum(m, best[u]);
     }
     if constexpr (S::kLanes == 8) m = max_dpp<0x140>(m);
-    m = max_xor(m, 16);
-    m = max_xor(m, 32);
-    const bool any_nan = __any(nan);
+    m = __builtin_elementwise_maximum(m, __shfl_xor(m, 16));
+    m = __builtin_elementwise_maximum(m, __shfl_xor(m, 32));
     again();
 
     const float ref = m == -kInf ? 0.f : m;
@@ -164,7 +160,8 @@ __global__ __launch_bounds__(256, 4) void spans_kernel(LogprobArgs a) {
         unpack(raw[u], f, (const T*)nullptr);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float d = __builtin_fmaf(fmaxf(f[i], -1e38f), kLog2e, -shift);
+          // the middle of three: a maximum in one instruction
+          const float d = __builtin_fmaf(__builtin_amdgcn_fmed3f(f[i], -1e38f, kInf), kLog2e, -shift);
           const float p = __builtin_amdgcn_exp2f(d);
           sum += p;
           weighted = __builtin_fmaf(p, d, weighted);
@@ -191,21 +188,7 @@ __global__ __launch_bounds__(256, 4) void spans_kernel(LogprobArgs a) {
         }
       }
     }
-    if (any_nan) {
-      again();
-#pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        float f[V];
-        unpack(raw[u], f, (const T*)nullptr);
-        int any = 0;
-#pragma unroll
-        for (int i = 0; i < V; ++i) any |= f[i] != f[i];
-#pragma unroll
-        for (int d = 1; d < S::kLanes; d <<= 1) any |= __shfl_xor(any, d);
-        if (any) best[u] = __builtin_nanf("");
-      }
-      m = sum = __builtin_nanf("");
-    }
+    if (m != m) sum = m;  // a NaN among the values: the row's
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       sum += __shfl_xor(sum, d);

@@ -12,9 +12,11 @@
 // magnitude of keys and values, settles both scales, re-rounds what the page
 // held where a scale grew, and writes the new codes, the values' by way of LDS,
 // where a tile of them is turned so that memory gets whole words of a column.
-// Bound by the bytes of the new tokens. Of single tokens, one wave owns a
-// sequence's head, half of it the key and half the value; bound by the chain of
-// loads from the length to the page's scale.
+// Bound by the bytes of the new tokens: 24.6 k tokens of 8 heads by 128 take 40
+// us, 3.8 TB/s read and written of the 4.9 that a large copy reaches. Of single
+// tokens, one wave owns a sequence's head, half of it the key and half the
+// value; 256 of them take 7 us, bound by the chain of loads from the length to
+// the page's scale.
 #include "device.h"
 #include "geometry.h"
 #include "serving.h"

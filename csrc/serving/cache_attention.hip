@@ -21,13 +21,13 @@
 // falls under fp16's range is under 2^-24 of the result. Sums are fp32.
 //
 // Of few rows, a workgroup's 4 waves take turns at tiles of 64 tokens and join
-// in LDS; of many, they have rows of their own and share the tiles. Long contexts are split over workgroups in chunks of a fixed number of tokens,
-// whose results a second launch joins in their order.
+// in LDS; of many, they have rows of their own and share the tiles. Long
+// contexts are split over workgroups in chunks of a fixed number of tokens, whose
+// results a second launch joins in their order.
 //
 // Measured, kernel and join: 64 contexts of 8000 to 16384 tokens, 64 heads on 8 of
-// 128: 280 + 8 us, 5.6 TB/s of the 6.3 that a plain read reaches (all heads of a
-// page on one die: 302 instead of 323 before the workgroups became fewer, see
-// split()); 32 of up to 4100 tokens: 34 + 5 us, bound by the latency of a
+// 128: 280 + 8 us, 5.7 TB/s of the 6.3 that a plain read reaches (all heads of a
+// page on one die took it from 323 to 302, fewer workgroups to 280: split()); 32 of up to 4100 tokens: 34 + 5 us, bound by the latency of a
 // workgroup's few tiles. A prompt of 4096 causal tokens, 32 heads on 8: 245 us,
 // 0.57 PFLOP/s; 4 chunks of 512 tokens on 8192: 350 us, 0.76 PFLOP/s, bound by the
 // vector unit's share of the softmax beside the matrix instructions.

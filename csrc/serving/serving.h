@@ -28,6 +28,7 @@ struct W4Args {
 int64_t w4_workspace(const W4Args& a);
 // Largest K: its scales and zero points have to fit the LDS.
 constexpr int kMaxColumns = 32768;
+constexpr int kMaxTokens = 65472;  // a grid's second dimension, in whole chunks
 hipError_t launch_w4_matmul(const W4Args& a, hipStream_t stream);
 
 // ---- 8-bit paged cache ----------------------------------------------------

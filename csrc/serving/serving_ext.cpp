@@ -344,6 +344,7 @@ PYBIND11_MODULE(_serving, m) {
   m.def("attention_places", &attention_places);
   m.def("append_places", &append_places);
   m.attr("MAX_COLUMNS") = kMaxColumns;
+  m.attr("MAX_TOKENS") = kMaxTokens;
   m.attr("MAX_TOP") = kMaxTop;
   m.attr("MAX_VOCAB") = kMaxVocab;
 }

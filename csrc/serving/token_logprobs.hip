@@ -13,9 +13,9 @@
 // Sums are fp32 over at most 4096 values a span, 64 a lane.
 //
 // 2048 x 130001 bf16, 5 alternatives: 110 us, 4.8 TB/s of the 6.3 that a plain
-// read reaches, and 10 us for the joins. What bounds it is the vector unit: 11
+// read reaches, and 11 us for the joins. What bounds it is the vector unit: 11
 // instructions a value, the exponential at a quarter of the rate, keep it busy
-// 88% of the time. One row of 32000 takes 4.4 us, and 12 us for its join with 20
+// 88% of the time. One row of 32000 takes 4.2 us, and 11 us for its join with 20
 // alternatives, a chain of dependent loads and selections in one workgroup.
 #include "device.h"
 #include "serving.h"

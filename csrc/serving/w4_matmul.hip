@@ -292,16 +292,15 @@ __global__ __launch_bounds__(W * 64) void w4_kernel(W4Args a, Tokens from) {
 }
 
 // Tokens in the order of the matrix instruction's loads, 1 KB for 16 tokens and
-// 32 columns; columns and tokens past the last are 0. A wave each.
+// 32 columns; columns and tokens past the last are 0. A thread has 8 columns of
+// a token, a wave 512 in a row, so that reads spread over the channels.
 template <typename T>
 __global__ __launch_bounds__(256) void pack_kernel(W4Args a, T* to, int mts, bool whole) {
   typedef typename Mat<T>::x8 x8;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int pieces = (a.k + 127) / 128 * 4 * mts;  // of a chunk of mts tiles
-  const int piece = blockIdx.x * 4 + wave;
-  if (piece >= pieces) return;
-  const int m = (blockIdx.y * mts + piece % mts) * 16 + (lane & 15);
-  const int k = piece / mts * 32 + (lane >> 4) * 8;
+  const int parts = (a.k + 127) / 128 * 16;  // of a token
+  const int part = blockIdx.x * 256 + threadIdx.x;
+  if (part >= parts) return;
+  const int m = blockIdx.y, k = part * 8;
   x8 v = bits_as<x8>(u32x4{0, 0, 0, 0});
   if (m < a.m) {
     const T* src = (const T*)a.x + m * a.ldx + k;
@@ -313,7 +312,9 @@ __global__ __launch_bounds__(256) void pack_kernel(W4Args a, T* to, int mts, boo
         if (k + i < a.k) v[i] = src[i];
     }
   }
-  *reinterpret_cast<x8*>(to + ((int64_t)blockIdx.y * pieces + piece) * 512 + lane * 8) = v;
+  const int chunk = m / (16 * mts), tile = m / 16 % mts;
+  const int64_t piece = (int64_t)chunk * (parts / 4) * mts + (int64_t)(part / 4) * mts + tile;
+  *reinterpret_cast<x8*>(to + piece * 512 + ((part % 4) * 16 + m % 16) * 8) = v;
 }
 
 int token_tiles(int m) { return m <= 16 ? 1 : m <= 32 ? 2 : 4; }
@@ -330,7 +331,7 @@ hipError_t launch(const W4Args& a, hipStream_t stream) {
   Tokens from{a.x, a.ldx, 0, 16 * MT * a.ldx, 32, 128, a.k, 0};
   if (!kX && packs(a)) {
     const int pieces = blocks * 4 * MT;
-    pack_kernel<T><<<dim3((pieces + 3) / 4, chunks), 256, 0, stream>>>(a, (T*)a.work, MT, whole_loads(a));
+    pack_kernel<T><<<dim3((blocks * 16 + 255) / 256, chunks * 16 * MT), 256, 0, stream>>>(a, (T*)a.work, MT, whole_loads(a));
     if (hipError_t e = hipGetLastError()) return e;
     from = Tokens{a.work, 8, 512, (int64_t)pieces * 512, MT * 512, MT * 2048, blocks * 128, 1};
   }

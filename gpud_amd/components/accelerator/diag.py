@@ -270,7 +270,7 @@ class ServingDiagComponent(_ManualDiagComponent):
     def __init__(self, inst: GPUdInstance):
         super().__init__(inst)
         self.gbps_floor = DEFAULT_SERVING_GBPS_FLOOR
-        self.iters = 50
+        self.steps = 50
 
     @property
     def name(self) -> str:
@@ -288,7 +288,7 @@ class ServingDiagComponent(_ManualDiagComponent):
             )
         failures, extra = [], {}
         for dev in range(ndev):
-            res = serving.serving_step(device=dev, iters=self.iters)
+            res = serving.serving_step(device=dev, iters=self.steps)
             extra[f"gpu{dev}.step_ms"] = f"{res['ms_per_step']:.3f}"
             extra[f"gpu{dev}.step_gbps"] = f"{res['gbps']:.0f}"
             extra[f"gpu{dev}.product_gbps"] = f"{res['product_gbps']:.0f}"

@@ -52,6 +52,7 @@ _MOST = 2**30
 
 GROUPS = (32, 64, 128)
 MAX_COLUMNS = _serving.MAX_COLUMNS
+MAX_TOKENS = _serving.MAX_TOKENS
 MAX_TOP = _serving.MAX_TOP
 MAX_VOCAB = _serving.MAX_VOCAB
 MAX_HEAD_DIM = 256
@@ -181,7 +182,8 @@ def w4_matmul(
     ``x`` is [M, K] in bf16 or fp16, its rows at any stride; ``codes``,
     ``scales`` (x's type) and ``zeros`` are as :func:`pack_w4` lays them out
     (no zeros: every zero point is 8). Meant for the tokens of a decode batch,
-    M up to 64; larger M are taken 64 rows at a time, K up to ``MAX_COLUMNS``.
+    M up to 64; larger M, up to ``MAX_TOKENS``, are taken 64 rows at a time,
+    and K up to ``MAX_COLUMNS``.
     Sums are fp32, rounded once to x's type. ``x`` has to be finite, and under 1e37 in magnitude.
     """
     dtype = _primary("x", x, 2, _HALVES)
@@ -189,7 +191,7 @@ def w4_matmul(
     n = int(out_features)
     if group_size not in GROUPS:
         raise ValueError(f"group_size must be one of {GROUPS}, not {group_size}")
-    if k < 1 or n < 1 or k > MAX_COLUMNS or n > _INT_MAX // 2 or m > 65535 * 16:
+    if k < 1 or n < 1 or k > MAX_COLUMNS or n > _INT_MAX // 2 or m > MAX_TOKENS:
         raise ValueError(f"no product of {m} rows with weights [{n}, {k}]")
     tiles, groups = -(-n // 16), -(-k // group_size)
     at, device = x.get_device(), x.device

@@ -180,6 +180,8 @@ def w4_args(**change):
         (dict(x=torch.zeros(256, dtype=BF16)), ValueError, "2 dimensions"),
         (dict(x=torch.zeros(3, 0, dtype=BF16)), ValueError, "no product"),
         (dict(x=torch.zeros(3, 300, dtype=BF16)), ValueError, "codes has shape"),
+        (dict(x=torch.zeros(1, 256, dtype=BF16).expand(65473, 256)), ValueError, "no product"),
+        (dict(x=torch.zeros(1, 32769, dtype=BF16)), ValueError, "no product"),
         (dict(out_features=0), ValueError, "no product"),
         (dict(out_features=33), ValueError, "codes has shape"),
         (dict(group_size=100), ValueError, "group_size"),

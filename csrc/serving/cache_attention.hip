@@ -96,8 +96,6 @@ struct Weighing {
   }
 };
 
-// DT tiles of 16 dimensions, all of them there if kWhole; QT tiles of 16 query
-// rows.
 // Codes that one workgroup reads once pass by the L2.
 template <int QT>
 __device__ __forceinline__ u32x4 load16(const uint8_t* p) {
@@ -115,6 +113,8 @@ __device__ __forceinline__ int anew(int v) {
 
 constexpr int waves_of(int dt, int qt) { return dt * qt <= 4 ? 3 : dt * qt <= 8 ? 2 : 1; }
 
+// DT tiles of 16 dimensions, all of them there if kWhole; QT tiles of 16 query
+// rows.
 template <typename T, int DT, int QT, bool kWhole>
 __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kernel(AttentionArgs a) {
   using x8 = typename Mat<T>::x8;

@@ -404,7 +404,10 @@ __global__ __launch_bounds__(kRow) void rows_kernel(LogprobArgs a) {
 template <typename T>
 hipError_t launch(const LogprobArgs& a, hipStream_t stream) {
   const Layout lay(a.vocab, Shape<T>::kSpan);
-  const dim3 grid((lay.spans + 3) / 4, a.rows < 65535 ? (int)a.rows : 65535);
+  const int across = (lay.spans + 3) / 4;
+  const int64_t down = (1 << 24) / across - 1;  // a launch has fewer than 2^32 threads
+  const int64_t most = down < 65535 ? down : 65535;
+  const dim3 grid(across, (unsigned)(a.rows < most ? a.rows : most));
   spans_kernel<T><<<grid, 256, 0, stream>>>(a);
   if (hipError_t e = hipGetLastError()) return e;
   const size_t lds = sizeof(uint64_t) * list_size(lay, a.top);

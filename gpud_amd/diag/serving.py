@@ -48,7 +48,13 @@ _HALVES = {torch.bfloat16: 0, torch.float16: 1}
 F8 = torch.float8_e4m3fn
 _CODES = (F8, torch.uint8)
 _INT_MAX = 2**31 - 1
-_MOST = 2**30
+_MOST = 2**30  # positions of a sequence
+# A launch has fewer than 2^32 threads in all; these sizes stay under it.
+_MOST_FEATURES = 2**26
+_MOST_PRODUCTS = 2**33
+_MOST_HEADS = 2**22  # heads of all sequences
+_MOST_HEAD_ROWS = 2**26  # (row, head) pairs
+_MOST_LOGIT_ROWS = 2**24 - 1
 
 GROUPS = (32, 64, 128)
 MAX_COLUMNS = _serving.MAX_COLUMNS
@@ -140,6 +146,8 @@ def pack_w4(
         raise ValueError(f"scales has shape {tuple(scales.shape)}; expected {(n, groups)}")
     if zeros is not None and tuple(zeros.shape) != (n, groups):
         raise ValueError(f"zeros has shape {tuple(zeros.shape)}; expected {(n, groups)}")
+    if zeros is not None and not torch.equal(zeros, zeros.round() if zeros.is_floating_point() else zeros):
+        raise ValueError("zeros must be whole numbers")
     for name, t in (("codes", codes), ("zeros", zeros)):
         if t is not None and (int(t.min()) < 0 or int(t.max()) > 15):
             raise ValueError(f"{name} must be in 0..15")
@@ -161,7 +169,9 @@ def pack_w4(
 
 def unpack_w4(packed: torch.Tensor, out_features: int, in_features: int) -> torch.Tensor:
     """The codes [N, K] (uint8) that :func:`pack_w4` laid out."""
-    tiles, blocks = packed.shape[:2]
+    _check_input("packed", packed, None, (torch.uint8,), 4)
+    tiles, blocks = -(-out_features // 16), -(-in_features // 128)
+    _check_shape("packed", packed, (tiles, blocks, 64, 16))
     nibbles = torch.stack((packed & 15, packed >> 4), -1).view(tiles, blocks, 4, 16, 4, 2, 4)
     full = nibbles.permute(0, 3, 1, 4, 2, 6, 5).reshape(tiles * 16, blocks * 128)
     return full[:out_features, :in_features].contiguous()
@@ -182,8 +192,9 @@ def w4_matmul(
     ``x`` is [M, K] in bf16 or fp16, its rows at any stride; ``codes``,
     ``scales`` (x's type) and ``zeros`` are as :func:`pack_w4` lays them out
     (no zeros: every zero point is 8). Meant for the tokens of a decode batch,
-    M up to 64; larger M, up to ``MAX_TOKENS``, are taken 64 rows at a time,
-    and K up to ``MAX_COLUMNS``.
+    M up to 64; larger M, up to ``MAX_TOKENS``, are taken 64 rows at a time.
+    K is at most ``MAX_COLUMNS``, N 2^26 and M N 2^33. ``out`` may not share
+    memory with the other arguments.
     Sums are fp32, rounded once to x's type. ``x`` has to be finite, and under 1e37 in magnitude.
     """
     dtype = _primary("x", x, 2, _HALVES)
@@ -191,7 +202,7 @@ def w4_matmul(
     n = int(out_features)
     if group_size not in GROUPS:
         raise ValueError(f"group_size must be one of {GROUPS}, not {group_size}")
-    if k < 1 or n < 1 or k > MAX_COLUMNS or n > _INT_MAX // 2 or m > MAX_TOKENS:
+    if k < 1 or n < 1 or k > MAX_COLUMNS or n > _MOST_FEATURES or m > MAX_TOKENS or m * n > _MOST_PRODUCTS:
         raise ValueError(f"no product of {m} rows with weights [{n}, {k}]")
     tiles, groups = -(-n // 16), -(-k // group_size)
     at, device = x.get_device(), x.device
@@ -295,8 +306,8 @@ def _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query
     if not _fits(seq_lens, at, torch.int32, (batch,)):
         _check_input("seq_lens", seq_lens, device, (torch.int32,), 1)
         _check_shape("seq_lens", seq_lens, (batch,))
-    if blocks * page > _MOST or batch * heads > _INT_MAX // 64:
-        raise ValueError("block_table covers more than 2^30 positions, or too many sequences and heads")
+    if blocks * page > _MOST or batch * heads > _MOST_HEADS:
+        raise ValueError("block_table covers more than 2^30 positions, or more than 2^22 heads of sequences")
     starts = 0
     if query_start is None:
         if rows != batch:
@@ -329,8 +340,9 @@ def cache_append(
     """Writes new keys and values [T, heads, dim] (bf16 or fp16) into the cache.
 
     Sequence b's new tokens are rows ``query_start[b] .. query_start[b+1]``
-    (int32 [B+1]), or row b alone without ``query_start``; they become its
-    last ones, and ``seq_lens`` (int32 [B]) counts them in. ``block_table``
+    (int32 [B+1], from 0 and never falling), or row b alone without
+    ``query_start``; they become its last ones, and ``seq_lens`` (int32 [B])
+    counts them in. ``block_table``
     (int32 [B, blocks]) names the page of each ``page_size`` positions. Rows
     may lie at any row and head stride.
 
@@ -339,7 +351,7 @@ def cache_append(
     again to it. A page whose first position is written starts afresh.
     Infinities are held as the largest code, NaN as NaN. Tokens whose page is
     out of range, or whose position is negative, are left out. A page that gets
-    tokens may belong to one sequence only.
+    tokens may stand in the table once only.
     """
     dtype = _primary("k", k, 3, _HALVES)
     device, at = k.device, k.get_device()
@@ -349,8 +361,8 @@ def cache_append(
     heads, dim, batch = cache[9], cache[11], cache[12]
     if k.shape != (rows, heads, dim) or v.shape != (rows, heads, dim):
         raise ValueError(f"k and v must be [T, {heads}, {dim}], not {tuple(k.shape)} and {tuple(v.shape)}")
-    if rows * heads > _MOST:
-        raise ValueError("more than 2^30 new keys")
+    if rows * heads > _MOST_HEAD_ROWS:
+        raise ValueError("more than 2^26 new keys")
     _check_gpu(device)
     if k.stride(2) != 1:
         k = k.contiguous()
@@ -393,7 +405,7 @@ def cache_attention(
     sees nothing gets 0 and -inf. A sequence whose pages are out of range, or
     that is longer than its row of ``block_table``, gets NaN. Rows behind the
     last sequence are left as they were in ``out`` if that is given, and else
-    0; their lse is -inf.
+    0; their lse is -inf. ``out`` may not share memory with the other arguments.
     """
     dtype = _primary("q", q, 3, _HALVES)
     device, at = q.device, q.get_device()
@@ -404,8 +416,8 @@ def cache_attention(
         raise ValueError(f"q has head dimension {dim}, the cache {cache[11]}")
     if q_heads < 1 or q_heads % heads or q_heads > 65535:
         raise ValueError(f"{q_heads} query heads do not share {heads} cached ones evenly")
-    if rows * q_heads > _MOST or batch * q_heads > _MOST:
-        raise ValueError("more than 2^30 query rows")
+    if rows * q_heads > _MOST_HEAD_ROWS or batch * q_heads > _MOST_HEAD_ROWS:
+        raise ValueError("more than 2^26 query rows")
     if scale is None:
         scale = dim**-0.5
     elif not 0 < scale < math.inf:
@@ -477,6 +489,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
     dtype = _primary("logits", logits, 2, _DTYPES)
     device, at = logits.device, logits.get_device()
     rows, vocab = logits.shape
+    if rows > _MOST_LOGIT_ROWS:
+        raise ValueError("more than 2^24 - 1 rows")
     if not _fits(targets, at, torch.int64, (rows,)):
         _check_input("targets", targets, device, (torch.int64,), 1)
         if targets.shape[0] != rows:
@@ -486,8 +500,6 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
         raise ValueError(f"vocabulary must have 1..{MAX_VOCAB} tokens, not {vocab}")
     if top_k < 0 or top_k > min(MAX_TOP, vocab):
         raise ValueError(f"top_k must be in 0..{min(MAX_TOP, vocab)}, not {top_k}")
-    if rows > _INT_MAX:
-        raise ValueError("more than 2^31 - 1 rows")
     _check_gpu(device)
     if logits.stride(1) != 1 and vocab > 1:
         logits = logits.contiguous()

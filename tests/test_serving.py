@@ -293,6 +293,45 @@ def test_token_logprobs_refuses(logits, targets, top, error, match):
         serving.token_logprobs(logits, targets, top)
 
 
+def many(*shape, dtype=BF16):
+    """A tensor of any size in the memory of one value."""
+    return torch.zeros(1, dtype=dtype).expand(*shape)
+
+
+def test_sizes_that_no_launch_can_have_are_refused():
+    codes, scales, _ = serving.pack_w4(torch.zeros(16, 16, dtype=torch.uint8), torch.zeros(16, 1, dtype=BF16))
+    for m, n in ((1, 2**26 + 1), (serving.MAX_TOKENS, 2**18)):
+        with pytest.raises(ValueError, match="no product"):
+            serving.w4_matmul(many(m, 16), codes, scales, out_features=n)
+    one = dict(block_table=torch.zeros(1, 5, dtype=torch.int32), seq_lens=torch.zeros(1, dtype=torch.int32))
+    one["query_start"] = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="new keys"):
+        serving.cache_append(many(2**25 + 1, 2, 64), many(2**25 + 1, 2, 64), **cache_args(**one))
+    with pytest.raises(ValueError, match="query rows"):
+        serving.cache_attention(many(2**24 + 1, 4, 64), **cache_args(**one))
+    batch = 2**21 + 1
+    lens, table = torch.zeros(batch, dtype=torch.int32), torch.zeros(batch, 1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="heads of sequences"):
+        serving.cache_attention(many(batch, 4, 64), **cache_args(block_table=table, seq_lens=lens))
+    with pytest.raises(ValueError, match="rows"):
+        serving.token_logprobs(many(2**24, 1), many(2**24, dtype=torch.long))
+
+
+def test_pack_w4_refuses_zero_points_between_whole_numbers():
+    codes, scales = torch.zeros(16, 16, dtype=torch.uint8), torch.ones(16, 1, dtype=BF16)
+    assert serving.pack_w4(codes, scales, torch.full((16, 1), 3.0))[2].unique().tolist() == [3]
+    with pytest.raises(ValueError, match="whole"):
+        serving.pack_w4(codes, scales, torch.full((16, 1), 3.5))
+
+
+def test_unpack_w4_refuses_other_sizes():
+    packed, _, _ = serving.pack_w4(torch.zeros(20, 130, dtype=torch.uint8), torch.zeros(20, 2, dtype=BF16))
+    assert serving.unpack_w4(packed, 20, 130).shape == (20, 130)
+    for n, k in ((33, 130), (16, 130), (20, 128), (20, 257)):
+        with pytest.raises(ValueError, match="packed"):
+            serving.unpack_w4(packed, n, k)
+
+
 def test_new_cache_refuses_sizes():
     for bad in ((0, 1, 64, 16), (1, 0, 64, 16), (1, 1, 65, 16), (1, 1, 64, 20), (1, 1, 64, 8)):
         with pytest.raises(ValueError):

@@ -15,8 +15,8 @@
 // before the fp32 sum of a group, which its scale multiplies.
 //
 // The 8 waves of a workgroup split the columns and join their sums in LDS, in
-// the waves' order, so that results do not depend on timing. 16 do where there
-// are fewer than 128 tiles of rows (54 x 170 x 7408: 22 us a pass instead of 31).
+// the waves' order, so that results do not depend on timing. 16 waves are slower
+// even where there are few tiles of rows (16 x 1024 x 8192: 12.5 us against 11.5).
 //
 // What the tokens cost beside the codes decides the rest (us, measured):
 // - Every load occupies the address path for 16 cycles, however little it
@@ -33,12 +33,17 @@
 //   tiles of tokens on (64 x 16384 x 8192: 30 + 2.5, against 45), but not for one
 //   (16 x 28672 x 8192: 28.5 + 2.5, against 30). It also takes rows that 16-byte
 //   loads do not fit.
+// - Workgroups that read the same tokens at the same time wait for the same
+//   channels: they start a block of columns apart (32 x 16384 x 8192: 23.4 with the
+//   packing, 26.3 without).
 // - The codes pass by the L2 (non-temporal): 5% at the largest sizes.
 #include "device.h"
 #include "serving.h"
 
 namespace serving {
 namespace {
+
+constexpr int W = 8;  // waves of a workgroup
 
 // 8 codes of a dword in the order of 8 consecutive columns, plus 16 each. The
 // instruction that masks and sets bits takes no constants: its mask lives in a
@@ -78,7 +83,7 @@ template <typename T, int MT, int NT>
 struct Lds {
   int groups, scales, zeros, x, pitch;  // bytes, and elements of a token's row
   size_t size;
-  __host__ __device__ Lds(const W4Args& a, bool with_x, int waves) {
+  __host__ __device__ Lds(const W4Args& a, bool with_x) {
     groups = (a.k + a.group - 1) / a.group;
     scales = NT * groups * 16 * (int)sizeof(T);
     zeros = a.zeros ? NT * groups * 16 : 0;
@@ -86,7 +91,7 @@ struct Lds {
     pitch = (a.k + 127) / 128 * 128 + 8;
     x = with_x ? (a.m < 16 * MT ? a.m : 16 * MT) * pitch * (int)sizeof(T) : 0;
     size = (size_t)scales + zeros + x;
-    const size_t sums = (size_t)waves * NT * MT * 1024;
+    const size_t sums = (size_t)W * NT * MT * 1024;
     if (size < sums) size = sums;
   }
 };
@@ -107,14 +112,17 @@ __device__ const u32x4 kNothing = {0, 0, 0, 0};
 
 // MT tiles of 16 tokens, NT tiles of 16 weight rows, groups of G columns. kX:
 // tokens come through LDS, else from memory.
-template <typename T, int MT, int NT, int G, bool kZeros, bool kX, int W>
+template <typename T, int MT, int NT, int G, bool kZeros, bool kX>
 __global__ __launch_bounds__(W * 64) void w4_kernel(W4Args a, Tokens from) {
   using x8 = typename Mat<T>::x8;
   typedef T t4 __attribute__((ext_vector_type(4)));
-  constexpr int kSubs = 128 / G;  // groups of a block of 128 columns
-  constexpr int kSteps = G / 32;  // matrix instructions of a group
+  // Of 64 tokens, groups of 128 columns are summed by halves, whose tokens are
+  // all in registers at once.
+  constexpr int kPart = MT > 2 && G > 64 ? 64 : G;
+  constexpr int kSubs = 128 / kPart;  // parts of a block of 128 columns
+  constexpr int kSteps = kPart / 32;  // matrix instructions of a part
   extern __shared__ u32x4 lds[];
-  const Lds<T, MT, NT> plan(a, kX, W);
+  const Lds<T, MT, NT> plan(a, kX);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 15, g = lane >> 4;
   const int tiles = (a.n + 15) >> 4, blocks = (a.k + 127) >> 7;
@@ -138,8 +146,8 @@ __global__ __launch_bounds__(W * 64) void w4_kernel(W4Args a, Tokens from) {
   }
   // The next turn's codes come from memory while this one's are at work, and
   // its tokens, kRing steps ahead, into the registers that a step leaves.
-  constexpr int kRing = kX || MT <= 2 ? 4 : 2;
-  constexpr bool kLate = kSteps > kRing;  // a group's tokens are never all here
+  constexpr bool kTurns = MT * NT > 8;
+  constexpr int kRing = kX || MT <= 2 || (kTurns && !kZeros) ? 4 : 2;
   u32x4 now[NT], next[NT];
   x8 xf[MT][kRing];
   auto load_codes = [&](int b) {
@@ -155,11 +163,15 @@ __global__ __launch_bounds__(W * 64) void w4_kernel(W4Args a, Tokens from) {
       xf[mt][j % kRing] = *reinterpret_cast<const x8*>(p);
     }
   };
+  // Turn i's block of columns. Of more than one tile of tokens, workgroups of a
+  // die begin a block apart, so that they do not all read the same tokens at once.
+  const int apart = MT > 1 ? (int)(blockIdx.x >> 3) % blocks : 0;
+  auto block_of = [&](int i) { return i + apart < blocks ? i + apart : i + apart - blocks; };
   if (wave < blocks) {
-    load_codes(wave);
+    load_codes(block_of(wave));
     if constexpr (!kX) {
 #pragma unroll
-      for (int j = 0; j < kRing; ++j) load_x(wave, j);
+      for (int j = 0; j < kRing; ++j) load_x(block_of(wave), j);
     }
   }
 
@@ -210,8 +222,9 @@ __global__ __launch_bounds__(W * 64) void w4_kernel(W4Args a, Tokens from) {
   const Decoder<T> decode;
   const x8 offset = splat8<T>(kZeros ? -16.f : -24.f);  // 24: 16 + 8
 #pragma unroll 1
-  for (int b = wave; b < blocks; b += W) {
-    const int after = b + W < blocks ? b + W : b;  // the last turn reads its own again
+  for (int turn = wave; turn < blocks; turn += W) {
+    const int b = block_of(turn);
+    const int after = block_of(turn + W < blocks ? turn + W : turn);  // the last turn reads its own again
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) now[nt] = next[nt];
     if constexpr (kX) {
@@ -223,34 +236,10 @@ __global__ __launch_bounds__(W * 64) void w4_kernel(W4Args a, Tokens from) {
     load_codes(after);
 #pragma unroll
     for (int s = 0; s < kSubs; ++s) {
-      int grp = b * kSubs + s;
+      int grp = b * (128 / G) + s * kPart / G;
       if (grp >= groups) grp = groups - 1;  // columns past the last: x is 0
-      f32x4 z[MT] = {}, part[NT][MT];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        if constexpr (!kLate) {
-#pragma unroll
-          for (int j = 0; j < kSteps; ++j) z[mt] = Mat<T>::mfma(offset, xf[mt][(s * kSteps + j) % kRing], z[mt]);
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) part[nt][mt] = z[mt];
-      }
-#pragma unroll
-      for (int j = s * kSteps; j < (s + 1) * kSteps; ++j) {
-        if constexpr (kLate) {
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) z[mt] = Mat<T>::mfma(offset, xf[mt][j % kRing], z[mt]);
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const x8 w = decode(now[nt][j]);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) part[nt][mt] = Mat<T>::mfma(w, xf[mt][j % kRing], part[nt][mt]);
-        }
-        if constexpr (!kX) load_x(j + kRing < 4 ? b : after, (j + kRing) % 4);
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      f32x4 z[MT] = {};
+      auto add = [&](int nt, const f32x4* part) {
         const int place = (nt * groups + grp) * 16 + g * 4;
         const t4 sc = bits_as<t4>(*reinterpret_cast<const u32x2*>(scales + place));
         uint32_t zp = 0;
@@ -259,13 +248,58 @@ __global__ __launch_bounds__(W * 64) void w4_kernel(W4Args a, Tokens from) {
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float v = kLate ? part[nt][mt][i] + z[mt][i] : part[nt][mt][i];
+            float v = part[mt][i];
             if constexpr (kZeros)  // z is -16 times the sum of x
               v = __builtin_fmaf((float)(zp >> (8 * i) & 255u), z[mt][i] * 0.0625f, v);
             acc[nt][mt][i] = __builtin_fmaf((float)sc[i], v, acc[nt][mt][i]);
           }
+      };
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) z[mt] = Mat<T>::mfma(offset, xf[mt][(s * kSteps + j) % kRing], z[mt]);
+      if constexpr (kTurns) {
+        // a tile of rows at a time, the sums of the one before being scaled
+        // meanwhile: those of all tiles at once take more registers than there are
+        f32x4 part[2][MT];
+#pragma unroll
+        for (int nt = 0; nt <= NT; ++nt) {
+          if (nt < NT) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) part[nt & 1][mt] = z[mt];
+#pragma unroll
+            for (int j = s * kSteps; j < (s + 1) * kSteps; ++j) {
+              const x8 w = decode(now[nt][j]);
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) part[nt & 1][mt] = Mat<T>::mfma(w, xf[mt][j % kRing], part[nt & 1][mt]);
+            }
+          }
+          if (nt > 0) add(nt - 1, part[nt - 1 & 1]);
+          if (nt == NT - 1) {
+#pragma unroll
+            for (int j = s * kSteps; j < (s + 1) * kSteps; ++j) load_x(j + kRing < 4 ? b : after, (j + kRing) % 4);
+          }
+        }
+      } else {
+        f32x4 part[NT][MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) part[nt][mt] = z[mt];
+#pragma unroll
+        for (int j = s * kSteps; j < (s + 1) * kSteps; ++j) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const x8 w = decode(now[nt][j]);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) part[nt][mt] = Mat<T>::mfma(w, xf[mt][j % kRing], part[nt][mt]);
+          }
+          if constexpr (!kX) load_x(j + kRing < 4 ? b : after, (j + kRing) % 4);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) add(nt, part[nt]);
       }
-      if constexpr (MT * NT > 4) __builtin_amdgcn_sched_barrier(0);  // registers
+      if constexpr (MT > 2 || MT * NT > 4) __builtin_amdgcn_sched_barrier(0);  // registers
     }
   }
 
@@ -324,7 +358,7 @@ bool packs(const W4Args& a) {
   return !through_lds(a) && (a.m > 16 || !whole_loads(a));
 }
 
-template <typename T, int MT, int NT, int G, bool kZeros, bool kX, int kWaves>
+template <typename T, int MT, int NT, int G, bool kZeros, bool kX>
 hipError_t launch(const W4Args& a, hipStream_t stream) {
   const int tiles = (a.n + 15) / 16, blocks = (a.k + 127) / 128;
   const int chunks = (a.m + 16 * MT - 1) / (16 * MT);
@@ -335,26 +369,26 @@ hipError_t launch(const W4Args& a, hipStream_t stream) {
     if (hipError_t e = hipGetLastError()) return e;
     from = Tokens{a.work, 8, 512, (int64_t)pieces * 512, MT * 512, MT * 2048, blocks * 128, 1};
   }
-  const Lds<T, MT, NT> plan(a, kX, kWaves);
-  auto kernel = w4_kernel<T, MT, NT, G, kZeros, kX, kWaves>;
+  const Lds<T, MT, NT> plan(a, kX);
+  auto kernel = w4_kernel<T, MT, NT, G, kZeros, kX>;
   if (plan.size > 65536) {
     const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)plan.size);
     if (e != hipSuccess) return e;
   }
-  kernel<<<dim3((tiles + NT - 1) / NT, chunks), kWaves * 64, plan.size, stream>>>(a, from);
+  kernel<<<dim3((tiles + NT - 1) / NT, chunks), W * 64, plan.size, stream>>>(a, from);
   return hipGetLastError();
 }
 
-template <typename T, int MT, int NT, bool kX, int W = 8>
+template <typename T, int MT, int NT, bool kX>
 hipError_t by_group(const W4Args& a, hipStream_t stream) {
   if (a.zeros) {
-    if (a.group == 32) return launch<T, MT, NT, 32, true, kX, W>(a, stream);
-    if (a.group == 64) return launch<T, MT, NT, 64, true, kX, W>(a, stream);
-    return launch<T, MT, NT, 128, true, kX, W>(a, stream);
+    if (a.group == 32) return launch<T, MT, NT, 32, true, kX>(a, stream);
+    if (a.group == 64) return launch<T, MT, NT, 64, true, kX>(a, stream);
+    return launch<T, MT, NT, 128, true, kX>(a, stream);
   }
-  if (a.group == 32) return launch<T, MT, NT, 32, false, kX, W>(a, stream);
-  if (a.group == 64) return launch<T, MT, NT, 64, false, kX, W>(a, stream);
-  return launch<T, MT, NT, 128, false, kX, W>(a, stream);
+  if (a.group == 32) return launch<T, MT, NT, 32, false, kX>(a, stream);
+  if (a.group == 64) return launch<T, MT, NT, 64, false, kX>(a, stream);
+  return launch<T, MT, NT, 128, false, kX>(a, stream);
 }
 
 template <typename T, int MT>
@@ -364,7 +398,6 @@ hipError_t by_rows(const W4Args& a, hipStream_t stream) {
   auto fits = [&](int nt) { return nt * ((a.k + a.group - 1) / a.group) * 48 <= 98304; };
   if (tiles >= 1024 && fits(4)) return by_group<T, MT, 4, false>(a, stream);
   if (tiles >= 512 && fits(2)) return by_group<T, MT, 2, false>(a, stream);
-  if (tiles < 128) return by_group<T, MT, 1, false, 16>(a, stream);
   return by_group<T, MT, 1, false>(a, stream);
 }
 

@@ -94,6 +94,20 @@ def test_w4_matmul(serving, m, n, k, group, zeros, dtype):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("zeros", (False, True))
+@pytest.mark.parametrize("group", (32, 64, 128))
+@pytest.mark.parametrize("n", (40, 8200, 16400))
+@pytest.mark.parametrize("m", (18, 50, 70))
+def test_w4_matmul_of_many_tokens(serving, m, n, group, zeros):
+    # 1, 2 and 4 tiles of rows a workgroup; the columns end inside a group, and
+    # there are fewer blocks of them than workgroups that begin apart
+    k, dtype = 1500, BF16 if m == 50 else FP16
+    x, (codes, scales, z), want, bound = w4_case(serving, m, n, k, group, zeros, dtype, seed=m + n + group)
+    got = serving.w4_matmul(x, codes, scales, z, out_features=n, group_size=group)
+    close(got, want, bound)
+    assert torch.equal(got, serving.w4_matmul(x, codes, scales, z, out_features=n, group_size=group))
+
+
 def test_w4_matmul_strides_offsets_and_out(serving):
     m, n, k = 5, 40, 256
     x, (codes, scales, z), want, bound = w4_case(serving, m, n, k, 64, True, BF16)

@@ -23,19 +23,24 @@
 //   fetches, as long as a load of 1 KB of codes. So scales and zero points come
 //   through LDS, and tokens too while they are under 32 KB in all: 1 x 28672 x
 //   8192 takes 24 with them in LDS, 29 without.
-// - Tokens that do not fit are read by every workgroup through the L2, so more
-//   than one tile of rows shares them where enough workgroups are left for the
-//   256 compute units: 4 tiles from 1024 on (64 x 16384 x 8192: 30, with two 37),
-//   2 from 512 on (5 x 8192 x 8192: 10.4; with one 11.3, with four 14.0), else 1
-//   (16 x 4096 x 4096: 7.7; with two 8.1).
+// - Tokens that do not fit are read by every workgroup through the L2, which is
+//   what a compute unit's second workgroup waits for: 16 x 8192 tokens by 256
+//   tiles of rows take 12.1, by 257 to 512 tiles 20.8, but with two tiles a
+//   workgroup 13.1. So one workgroup a unit has all its tiles, up to 8 (16 x 28672
+//   x 8192: 28; with four tiles, 448 workgroups, 34), 4 of 64 tokens. Of fewer than
+//   8 tokens, two workgroups with a tile each take 9.5, one with two 10.2 (5 x 5000
+//   x 5000). Tokens in LDS: two tiles a workgroup from 512 tiles on (1 x 28672 x
+//   8192: 25.8, with one 27.8; 1 x 8192 x 8192: 10.5 and 9.7).
 // - Rows of tokens a power of two apart fall on the same channels of the L2. A
 //   launch before lays tokens out in the order of the loads, which pays from two
-//   tiles of tokens on (64 x 16384 x 8192: 30 + 2.5, against 45), but not for one
-//   (16 x 28672 x 8192: 28.5 + 2.5, against 30). It also takes rows that 16-byte
+//   tiles of tokens on (64 x 16384 x 8192: 34 with it, 44 without), but not for one
+//   (16 x 28672 x 8192: 29.5 with it, 28 without). It also takes rows that 16-byte
 //   loads do not fit.
-// - Workgroups that read the same tokens at the same time wait for the same
-//   channels: they start a block of columns apart (32 x 16384 x 8192: 23.4 with the
-//   packing, 26.3 without).
+// - Workgroups that read the same tokens, or rows of weights a power of two apart,
+//   at the same time wait for the same channels: they start a block of columns
+//   apart (32 x 16384 x 8192: 23.4 with the packing, 26.3 without; 16 x 32768 x
+//   8192: 31.4, 36.7). For one tile of tokens and few tiles of rows it only costs
+//   (16 x 8192 x 8192: 13.8 instead of 13.2).
 // - The codes pass by the L2 (non-temporal): 5% at the largest sizes.
 #include "device.h"
 #include "serving.h"
@@ -163,9 +168,9 @@ __global__ __launch_bounds__(W * 64) void w4_kernel(W4Args a, Tokens from) {
       xf[mt][j % kRing] = *reinterpret_cast<const x8*>(p);
     }
   };
-  // Turn i's block of columns. Of more than one tile of tokens, workgroups of a
-  // die begin a block apart, so that they do not all read the same tokens at once.
-  const int apart = MT > 1 ? (int)(blockIdx.x >> 3) % blocks : 0;
+  // Turn i's block of columns: where it pays, workgroups of a die begin a block
+  // apart.
+  const int apart = MT > 1 || NT % 4 == 0 ? (int)(blockIdx.x >> 3) % blocks : 0;
   auto block_of = [&](int i) { return i + apart < blocks ? i + apart : i + apart - blocks; };
   if (wave < blocks) {
     load_codes(block_of(wave));
@@ -391,19 +396,43 @@ hipError_t by_group(const W4Args& a, hipStream_t stream) {
   return launch<T, MT, NT, 128, false, kX>(a, stream);
 }
 
+// Tiles of rows of a workgroup: as many as let one round of workgroups, one for
+// each compute unit, do, and in more rounds as few as leave those even. The
+// tokens of up to 7 rows cost little enough for two workgroups a unit.
+template <int kMost>
+int row_tiles(const W4Args& a) {
+  const int tiles = (a.n + 15) / 16, units = 256;
+  if (a.m < 8 && tiles <= 2 * units) return 1;
+  // their scales have to leave room in the LDS
+  const int fit = 147456 / ((a.k + a.group - 1) / a.group * 48);
+  const int most = fit < 1 ? 1 : fit < kMost ? fit : kMost;
+  const int rounds = (tiles + units * most - 1) / (units * most);
+  return (tiles + units * rounds - 1) / (units * rounds);
+}
+
 template <typename T, int MT>
 hipError_t by_rows(const W4Args& a, hipStream_t stream) {
-  const int tiles = (a.n + 15) / 16;
-  // scales of more tiles than one have to leave room in the LDS
-  auto fits = [&](int nt) { return nt * ((a.k + a.group - 1) / a.group) * 48 <= 98304; };
-  if (tiles >= 1024 && fits(4)) return by_group<T, MT, 4, false>(a, stream);
-  if (tiles >= 512 && fits(2)) return by_group<T, MT, 2, false>(a, stream);
-  return by_group<T, MT, 1, false>(a, stream);
+  constexpr int kMost = MT > 2 ? 4 : 8;  // registers
+  switch (row_tiles<kMost>(a)) {
+    case 1: return by_group<T, MT, 1, false>(a, stream);
+    case 2: return by_group<T, MT, 2, false>(a, stream);
+    case 3: return by_group<T, MT, 3, false>(a, stream);
+    case 4: return by_group<T, MT, 4, false>(a, stream);
+  }
+  if constexpr (kMost > 4) {
+    switch (row_tiles<kMost>(a)) {
+      case 5: return by_group<T, MT, 5, false>(a, stream);
+      case 6: return by_group<T, MT, 6, false>(a, stream);
+      case 7: return by_group<T, MT, 7, false>(a, stream);
+      case 8: return by_group<T, MT, 8, false>(a, stream);
+    }
+  }
+  return hipErrorInvalidValue;
 }
 
 template <typename T>
 hipError_t by_tokens(const W4Args& a, hipStream_t stream) {
-  if (through_lds(a)) return by_group<T, 1, 1, true>(a, stream);
+  if (through_lds(a)) return a.n > 8192 ? by_group<T, 1, 2, true>(a, stream) : by_group<T, 1, 1, true>(a, stream);
   switch (token_tiles(a.m)) {
     case 1: return by_rows<T, 1>(a, stream);
     case 2: return by_rows<T, 2>(a, stream);

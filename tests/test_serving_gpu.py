@@ -108,6 +108,26 @@ def test_w4_matmul_of_many_tokens(serving, m, n, group, zeros):
     assert torch.equal(got, serving.w4_matmul(x, codes, scales, z, out_features=n, group_size=group))
 
 
+@pytest.mark.parametrize("zeros", (False, True))
+@pytest.mark.parametrize("group", (32, 64, 128))
+@pytest.mark.parametrize("tiles", (257, 520, 770, 1030, 1300, 1788, 1794, 2100))
+@pytest.mark.parametrize("m", (2, 16, 29, 61))
+def test_w4_matmul_of_any_number_of_rows(serving, m, tiles, group, zeros):
+    # from 1 to 8 tiles of rows a workgroup, the last of them not there or not whole
+    n, k, dtype = tiles * 16 - 5, 1100, FP16 if m == 16 else BF16
+    x, (codes, scales, z), want, bound = w4_case(serving, m, n, k, group, zeros, dtype, seed=m + n + group)
+    close(serving.w4_matmul(x, codes, scales, z, out_features=n, group_size=group), want, bound)
+
+
+def test_w4_matmul_of_the_most_columns(serving):
+    # as many scales and zero points as the LDS holds
+    n, k = 16 * 600, serving.MAX_COLUMNS
+    for m in (1, 16, 40):
+        x, (codes, scales, z), want, bound = w4_case(serving, m, n, k, 32, True, BF16, seed=m)
+        close(serving.w4_matmul(x, codes, scales, z, out_features=n, group_size=32), want, bound)
+        del want, bound
+
+
 def test_w4_matmul_strides_offsets_and_out(serving):
     m, n, k = 5, 40, 256
     x, (codes, scales, z), want, bound = w4_case(serving, m, n, k, 64, True, BF16)

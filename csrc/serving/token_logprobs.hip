@@ -15,8 +15,8 @@
 // 2048 x 130001 bf16, 5 alternatives: 110 us, 4.8 TB/s of the 6.3 that a plain
 // read reaches, and 11 us for the joins. What bounds it is the vector unit: 11
 // instructions a value, the exponential at a quarter of the rate, keep it busy
-// 88% of the time. One row of 32000 takes 4.2 us, and 11 us for its join with 20
-// alternatives, a chain of dependent loads and selections in one workgroup.
+// 88% of the time. One row of 32000 with 20 alternatives takes 10.5 us, most of them
+// for its join, a chain of dependent loads and selections in one workgroup.
 #include "device.h"
 #include "serving.h"
 
@@ -93,130 +93,134 @@ __device__ __forceinline__ float value_of(uint32_t order) {
   return bits_as<float>(order & 0x80000000u ? order & 0x7FFFFFFFu : ~order);  // all ones: NaN
 }
 
+// A wave's span of a row, left in row `at` of `work`.
 template <typename T>
-__global__ __launch_bounds__(256, 5) void spans_kernel(LogprobArgs a) {
+__device__ __forceinline__ void take_span(const LogprobArgs& a, const Layout& lay, int64_t row, int span, float* work, int64_t at) {
   using S = Shape<T>;
   constexpr int V = S::kVec;
-  const Layout lay(a.vocab, S::kSpan);
   const int lane = threadIdx.x & 63;
-  const int span = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (span >= lay.spans) return;
-  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
-    const T* x = (const T*)a.logits + row * a.ld;
-    const int shift = (int)(((uintptr_t)x / sizeof(T)) % V);
-    const int first = span * S::kSpan + lane * V - shift;  // index of the lane's first value
+  const T* x = (const T*)a.logits + row * a.ld;
+  const int shift = (int)(((uintptr_t)x / sizeof(T)) % V);
+  const int first = span * S::kSpan + lane * V - shift;  // index of the lane's first value
 
-    u32x4 raw[kUnits];
-    if (span * S::kSpan - shift >= 0 && (span + 1) * S::kSpan - shift <= a.vocab) {
+  u32x4 raw[kUnits];
+  if (span * S::kSpan - shift >= 0 && (span + 1) * S::kSpan - shift <= a.vocab) {
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) raw[u] = *reinterpret_cast<const u32x4*>(x + first + u * 64 * V);
-    } else {
+    for (int u = 0; u < kUnits; ++u) raw[u] = *reinterpret_cast<const u32x4*>(x + first + u * 64 * V);
+  } else {
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        const int e = first + u * 64 * V;
-        if (e >= 0 && e + V <= a.vocab) {
-          raw[u] = *reinterpret_cast<const u32x4*>(x + e);
-        } else {  // the row's ends: nothing outside it is read
-          T part[V];
+    for (int u = 0; u < kUnits; ++u) {
+      const int e = first + u * 64 * V;
+      if (e >= 0 && e + V <= a.vocab) {
+        raw[u] = *reinterpret_cast<const u32x4*>(x + e);
+      } else {  // the row's ends: nothing outside it is read
+        T part[V];
 #pragma unroll
-          for (int i = 0; i < V; ++i) part[i] = (e + i >= 0 && e + i < a.vocab) ? x[e + i] : (T)-kInf;
-          __builtin_memcpy(&raw[u], part, 16);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < V; ++i) part[i] = (e + i >= 0 && e + i < a.vocab) ? x[e + i] : (T)-kInf;
+        __builtin_memcpy(&raw[u], part, 16);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    const int64_t t = a.targets[row];
-    const bool known = t >= 0 && t < a.vocab;
-    const float xt = known ? (float)x[t] : kInf;
+  }
+  const int64_t t = a.targets[row];
+  const bool known = t >= 0 && t < a.vocab;
+  const float xt = known ? (float)x[t] : kInf;
 
-    // The two passes over the registers unpack them anew: kept, the values
-    // would take the registers of three waves in five.
-    auto again = [&] {
+  // The two passes over the registers unpack them anew: kept, the values
+  // would take the registers of three waves in five.
+  auto again = [&] {
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) asm volatile("" : "+v"(raw[u]));
-    };
-    float best[kUnits];  // of the lane's group of 64 values
-    float m = -kInf;
+    for (int u = 0; u < kUnits; ++u) asm volatile("" : "+v"(raw[u]));
+  };
+  float best[kUnits];  // of the lane's group of 64 values
+  float m = -kInf;
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    float f[V];
+    unpack(raw[u], f, (const T*)nullptr);
+    float b = f[0];
+#pragma unroll
+    for (int i = 1; i < V; ++i) b = __builtin_elementwise_maximum(b, f[i]);  // a NaN stays
+    best[u] = group_max<S::kLanes>(b);
+    m = __builtin_elementwise_maximum(m, best[u]);
+  }
+  if constexpr (S::kLanes == 8) m = max_dpp<0x140>(m);
+  m = __builtin_elementwise_maximum(m, __shfl_xor(m, 16));
+  m = __builtin_elementwise_maximum(m, __shfl_xor(m, 32));
+  again();
+
+  const float ref = m == -kInf ? 0.f : m;
+  float sum = 0.f, weighted = 0.f;
+  int above = 0;
+  if (fabsf(ref) < 1e37f) {
+    // u = x log2 e - m log2 e in one step. The product with m is off by a
+    // rounding, the same for all values, and comes off the sums again; what
+    // lies below -1e38 (masks, -inf) is at 0 either way.
+    const float shift = ref * kLog2e, off = __builtin_fmaf(ref, kLog2e, -shift);
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       float f[V];
       unpack(raw[u], f, (const T*)nullptr);
-      float b = f[0];
 #pragma unroll
-      for (int i = 1; i < V; ++i) b = __builtin_elementwise_maximum(b, f[i]);  // a NaN stays
-      best[u] = group_max<S::kLanes>(b);
-      m = __builtin_elementwise_maximum(m, best[u]);
-    }
-    if constexpr (S::kLanes == 8) m = max_dpp<0x140>(m);
-    m = __builtin_elementwise_maximum(m, __shfl_xor(m, 16));
-    m = __builtin_elementwise_maximum(m, __shfl_xor(m, 32));
-    again();
-
-    const float ref = m == -kInf ? 0.f : m;
-    float sum = 0.f, weighted = 0.f;
-    int above = 0;
-    if (fabsf(ref) < 1e37f) {
-      // u = x log2 e - m log2 e in one step. The product with m is off by a
-      // rounding, the same for all values, and comes off the sums again; what
-      // lies below -1e38 (masks, -inf) is at 0 either way.
-      const float shift = ref * kLog2e, off = __builtin_fmaf(ref, kLog2e, -shift);
-#pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        float f[V];
-        unpack(raw[u], f, (const T*)nullptr);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          // the middle of three: a maximum in one instruction
-          const float d = __builtin_fmaf(__builtin_amdgcn_fmed3f(f[i], -1e38f, kInf), kLog2e, -shift);
-          const float p = __builtin_amdgcn_exp2f(d);
-          sum += p;
-          weighted = __builtin_fmaf(p, d, weighted);
-          above += __popcll(__ballot(f[i] > xt));
-        }
-        __builtin_amdgcn_sched_barrier(0);  // registers
+      for (int i = 0; i < V; ++i) {
+        // the middle of three: a maximum in one instruction
+        const float d = __builtin_fmaf(__builtin_amdgcn_fmed3f(f[i], -1e38f, kInf), kLog2e, -shift);
+        const float p = __builtin_amdgcn_exp2f(d);
+        sum += p;
+        weighted = __builtin_fmaf(p, d, weighted);
+        above += __popcll(__ballot(f[i] > xt));
       }
-      const float back = __builtin_amdgcn_exp2f(-off);
-      weighted = (weighted - off * sum) * back;
-      sum *= back;
-      if (m == -kInf) sum = weighted = 0.f;
-    } else {
+      __builtin_amdgcn_sched_barrier(0);  // registers
+    }
+    const float back = __builtin_amdgcn_exp2f(-off);
+    weighted = (weighted - off * sum) * back;
+    sum *= back;
+    if (m == -kInf) sum = weighted = 0.f;
+  } else {
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        float f[V];
-        unpack(raw[u], f, (const T*)nullptr);
+    for (int u = 0; u < kUnits; ++u) {
+      float f[V];
+      unpack(raw[u], f, (const T*)nullptr);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float d = (f[i] - ref) * kLog2e;
-          const float p = __builtin_amdgcn_exp2f(d);
-          sum += p;
-          weighted = __builtin_fmaf(p, fmaxf(d, -256.f), weighted);  // 2^-256 is 0: no 0 x inf
-          above += __popcll(__ballot(f[i] > xt));
-        }
+      for (int i = 0; i < V; ++i) {
+        const float d = (f[i] - ref) * kLog2e;
+        const float p = __builtin_amdgcn_exp2f(d);
+        sum += p;
+        weighted = __builtin_fmaf(p, fmaxf(d, -256.f), weighted);  // 2^-256 is 0: no 0 x inf
+        above += __popcll(__ballot(f[i] > xt));
       }
-    }
-    if (m != m) sum = m;  // a NaN among the values: the row's
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      sum += __shfl_xor(sum, d);
-      weighted += __shfl_xor(weighted, d);
-    }
-    if (lane == 0) {
-      f32x4 s;
-      s[0] = m == -kInf ? -kInf : ref;
-      s[1] = sum;
-      s[2] = weighted;
-      s[3] = bits_as<float>(above);
-      float* to = lay.stats(a.work, row, span);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) to[i] = s[i];
-      lay.tops(a.work, row)[span] = m;
-    }
-    if (a.top && lane % S::kLanes == 0) {
-      float* to = lay.group(a.work, row, span) + lane / S::kLanes;
-#pragma unroll
-      for (int u = 0; u < kUnits; ++u) to[u * (64 / S::kLanes)] = best[u];
     }
   }
+  if (m != m) sum = m;  // a NaN among the values: the row's
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    sum += __shfl_xor(sum, d);
+    weighted += __shfl_xor(weighted, d);
+  }
+  if (lane == 0) {
+    f32x4 s;
+    s[0] = m == -kInf ? -kInf : ref;
+    s[1] = sum;
+    s[2] = weighted;
+    s[3] = bits_as<float>(above);
+    float* to = lay.stats(work, at, span);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i] = s[i];
+    lay.tops(work, at)[span] = m;
+  }
+  if (a.top && lane % S::kLanes == 0) {
+    float* to = lay.group(work, at, span) + lane / S::kLanes;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) to[u * (64 / S::kLanes)] = best[u];
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256, 5) void spans_kernel(LogprobArgs a) {
+  const Layout lay(a.vocab, Shape<T>::kSpan);
+  const int span = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (span >= lay.spans) return;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) take_span<T>(a, lay, row, span, a.work, row);
 }
 
 // Lists of (order, place) in LDS, one list a wave; a key is larger where the
@@ -236,37 +240,53 @@ __device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t place) {
 
 constexpr int kRow = 256;  // threads of a row's join
 
+// What select_top() needs in LDS.
+struct Selection {
+  uint64_t most[kRow];
+  int place[kRow];
+  int counts[kRow / 64];
+};
+
 // Sorts out the `want` largest of list[0..n), all different, into out[0..want)
-// in falling order; list is used up, `most` holds kRow keys. All kRow threads.
-__device__ void select_top(uint64_t* list, int n, int want, uint64_t* out, uint64_t* most, int* counts) {
+// in falling order; list is used up. All kRow threads.
+__device__ void select_top(uint64_t* list, int n, int want, uint64_t* out, Selection& use) {
   const int me = threadIdx.x, wave = me >> 6;
   if (n > kRow) {
-    // The want-th largest of the threads' largest is a floor under the want
-    // largest of all, and seldom far under them. A thread has n / kRow keys, so
-    // at most want times that are left, 1024.
+    // Of `lists` lists, the want-th of their largest is a floor under the want
+    // largest of all, and seldom far under them where lists are three times as
+    // many or more. Its search costs lists^2 / kRow steps, so there are no more.
+    const int lists = want <= 24 ? 64 : want <= 48 ? 128 : 256;
+    const int id = me & (lists - 1);
     uint64_t mine = 0;
     for (int i = me; i < n; i += kRow) mine = list[i] > mine ? list[i] : mine;
-    most[me] = mine;
+    use.most[me] = mine;
+    use.place[me] = 0;
     __syncthreads();
+    for (int i = id; i < kRow; i += lists) mine = use.most[i] > mine ? use.most[i] : mine;
+    __syncthreads();
+    if (me < lists) use.most[me] = mine;
+    __syncthreads();
+    const int share = lists * lists / kRow, first = me / lists * share;
     int place = 0;
 #pragma unroll 8
-    for (int j = 0; j < kRow; ++j) place += most[j] > mine;
+    for (int j = 0; j < share; ++j) place += use.most[first + j] > mine;
+    atomicAdd(&use.place[id], place);
     __syncthreads();
-    if (place == want - 1) most[0] = mine;
+    if (me < lists && use.place[me] == want - 1) use.most[0] = mine;
     __syncthreads();
-    const uint64_t low = most[0];
+    const uint64_t low = use.most[0];
     int kept = 0;
     for (int i = 0; i < n; i += kRow) {
       const uint64_t key = i + me < n ? list[i + me] : 0;
       const bool in = i + me < n && key >= low;
       const uint64_t mask = __ballot(in);
-      if ((me & 63) == 0) counts[wave] = __popcll(mask);
+      if ((me & 63) == 0) use.counts[wave] = __popcll(mask);
       __syncthreads();  // also: every thread has read this part of the list
       int at = kept;
 #pragma unroll
       for (int w = 0; w < kRow / 64; ++w) {
-        if (w < wave) at += counts[w];
-        kept += counts[w];
+        if (w < wave) at += use.counts[w];
+        kept += use.counts[w];
       }
       if (in) list[at + __popcll(mask & ((1ull << (me & 63)) - 1))] = key;
       __syncthreads();
@@ -282,28 +302,32 @@ __device__ void select_top(uint64_t* list, int n, int want, uint64_t* out, uint6
   }
 }
 
+// Joins the spans of a row, left in row `from` of `work`. All kRow threads; 64 do
+// if there are no alternatives to find.
 template <typename T>
-__global__ __launch_bounds__(kRow) void rows_kernel(LogprobArgs a) {
+__device__ __forceinline__ void join_row(const LogprobArgs& a, const Layout& lay, int64_t row, float* work, int64_t from_row) {
   using S = Shape<T>;
-  const Layout lay(a.vocab, S::kSpan);
   const int me = threadIdx.x, lane = me & 63, wave = me >> 6;
-  const int64_t row = blockIdx.x;
   const T* x = (const T*)a.logits + row * a.ld;
+  const int64_t t = a.targets[row];  // early: two loads that wait for one another
+  const bool known = t >= 0 && t < a.vocab;
+  const float xt = known ? (float)x[t] : 0.f;
 
   extern __shared__ uint64_t list[];  // list_size()
-  __shared__ uint64_t out[3][kMaxTop], most[kRow];
-  __shared__ int counts[kRow / 64];
+  __shared__ uint64_t out[3][kMaxTop];
+  __shared__ Selection use;
+  __shared__ int found;
   // groups of 64 where they are few enough to go through at once, else spans
   const bool direct = (int64_t)lay.spans * lay.groups <= kDirect;
   int n = direct ? lay.spans * lay.groups : lay.spans;
   if (a.top) {
-    const float* from = direct ? lay.group(a.work, row, 0) : lay.tops(a.work, row);
+    const float* from = direct ? lay.group(work, from_row, 0) : lay.tops(work, from_row);
     for (int i = me; i < n; i += kRow) list[i] = key_of(order_of(from[i]), i);
   }
 
   // the spans' sums against one reference, each lane's in the spans' order; all
   // waves alike
-  const float* stats = lay.stats(a.work, row, 0);
+  const float* stats = lay.stats(work, from_row, 0);
   float ref = -kInf;
   for (int s = lane; s < lay.spans; s += 64) ref = fmaxf(ref, stats[s * 4]);
 #pragma unroll
@@ -329,9 +353,7 @@ __global__ __launch_bounds__(kRow) void rows_kernel(LogprobArgs a) {
   const bool empty = ref == -kInf && !(sum != sum);  // every token masked
   auto logp = [&](float v) { return empty ? -kInf : (v - ref) - log_sum; };
   if (me == 0) {
-    const int64_t t = a.targets[row];
-    const bool known = t >= 0 && t < a.vocab;
-    a.logprob[row] = known ? logp((float)x[t]) : t < 0 ? 0.f : __builtin_nanf("");
+    a.logprob[row] = known ? logp(xt) : t < 0 ? 0.f : __builtin_nanf("");
     a.entropy[row] = empty ? 0.f : log_sum - weighted / sum * kLn2;
     a.rank[row] = known ? above : -1;
   }
@@ -350,7 +372,7 @@ __global__ __launch_bounds__(kRow) void rows_kernel(LogprobArgs a) {
       const int size = level == 1 ? S::kGroups : 64;
       const uint32_t least = parts == want ? (uint32_t)(out[level - 1][parts - 1] >> 32) : 0u;
       constexpr int kBatch = 4;
-      if (me == 0) counts[0] = 0;
+      if (me == 0) found = 0;
       __syncthreads();
 #pragma unroll 1
       for (int first = wave; first < parts; first += kBatch * (kRow / 64)) {
@@ -365,7 +387,7 @@ __global__ __launch_bounds__(kRow) void rows_kernel(LogprobArgs a) {
           in[q] = p < parts && lane < size && (level == 1 || place[q] < (uint32_t)a.vocab);
         }
         if (level == 1) {
-          const float* from = lay.group(a.work, row, 0);
+          const float* from = lay.group(work, from_row, 0);
 #pragma unroll
           for (int q = 0; q < kBatch; ++q) value[q] = from[in[q] ? place[q] : 0];
         } else {
@@ -381,17 +403,17 @@ __global__ __launch_bounds__(kRow) void rows_kernel(LogprobArgs a) {
           const bool kept = in[q] && order >= least;
           const uint64_t mask = __ballot(kept);
           int at = 0;
-          if (lane == 0 && mask) at = atomicAdd(&counts[0], __popcll(mask));
+          if (lane == 0 && mask) at = atomicAdd(&found, __popcll(mask));
           at = __builtin_amdgcn_readfirstlane(at);
           if (kept) list[at + __popcll(mask & ((1ull << lane) - 1))] = key_of(order, place[q]);
         }
       }
       __syncthreads();
-      n = counts[0];
+      n = found;
     }
     __syncthreads();
     got = n < want ? n : want;
-    select_top(list, n, got, out[level], most, counts);
+    select_top(list, n, got, out[level], use);
     __syncthreads();
   }
   for (int i = me; i < want; i += kRow) {
@@ -402,15 +424,46 @@ __global__ __launch_bounds__(kRow) void rows_kernel(LogprobArgs a) {
 }
 
 template <typename T>
+__global__ __launch_bounds__(kRow) void rows_kernel(LogprobArgs a) {
+  const Layout lay(a.vocab, Shape<T>::kSpan);
+  join_row<T>(a, lay, blockIdx.x, a.work, blockIdx.x);
+}
+
+// Few rows of few spans: a workgroup takes a row's spans, a wave each, and joins
+// them from the LDS, which saves a launch and the workspace (a pass of 256 x 32000
+// bf16 with 20 alternatives: 13.1 us, 257 rows in two launches 18.0). Of more rows
+// than compute units, workgroups wait for the joins of others (512 x 1000: 25.8 in
+// one launch, 17.3 in two), and with two spans a wave a row is slower too (1 x
+// 130001: 23.9, 17.1). Both ways compute the same.
+constexpr int kFewSpans = 16;
+template <typename T>
+__global__ __launch_bounds__(kFewSpans * 64) void row_kernel(LogprobArgs a) {
+  using S = Shape<T>;
+  __shared__ float work[kFewSpans * (5 + S::kGroups)];
+  const Layout lay(a.vocab, S::kSpan);
+  const int wave = threadIdx.x >> 6;
+  if (wave < lay.spans) take_span<T>(a, lay, blockIdx.x, wave, work, 0);
+  __syncthreads();
+  if (wave >= kRow / 64) return;  // barriers wait for the waves that are left
+  join_row<T>(a, lay, blockIdx.x, work, 0);
+}
+
+bool in_one(int64_t rows, const Layout& lay) { return rows <= 256 && lay.spans <= kFewSpans; }
+
+template <typename T>
 hipError_t launch(const LogprobArgs& a, hipStream_t stream) {
   const Layout lay(a.vocab, Shape<T>::kSpan);
+  const size_t lds = sizeof(uint64_t) * list_size(lay, a.top);
+  if (in_one(a.rows, lay)) {
+    row_kernel<T><<<dim3((unsigned)a.rows), kFewSpans * 64, lds, stream>>>(a);
+    return hipGetLastError();
+  }
   const int across = (lay.spans + 3) / 4;
   const int64_t down = (1 << 24) / across - 1;  // a launch has fewer than 2^32 threads
   const int64_t most = down < 65535 ? down : 65535;
   const dim3 grid(across, (unsigned)(a.rows < most ? a.rows : most));
   spans_kernel<T><<<grid, 256, 0, stream>>>(a);
   if (hipError_t e = hipGetLastError()) return e;
-  const size_t lds = sizeof(uint64_t) * list_size(lay, a.top);
   rows_kernel<T><<<dim3((unsigned)a.rows), a.top ? kRow : 64, lds, stream>>>(a);
   return hipGetLastError();
 }
@@ -419,7 +472,8 @@ hipError_t launch(const LogprobArgs& a, hipStream_t stream) {
 
 int64_t logprob_workspace(int64_t rows, int vocab, int dtype) {
   const int span = dtype == kF32 ? Shape<float>::kSpan : Shape<__bf16>::kSpan;
-  return rows * Layout(vocab, span).row;
+  const Layout lay(vocab, span);
+  return in_one(rows, lay) ? 0 : rows * lay.row;
 }
 
 hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t stream) {

@@ -510,10 +510,11 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
     if top_k:
         top_ids, top_logprobs = rank.new_empty((rows, top_k)), logprob.new_empty((rows, top_k))
     if rows:
-        work = logprob.new_empty(_serving.logprob_workspace(rows, vocab, dtype))
+        floats = _serving.logprob_workspace(rows, vocab, dtype)
+        work = logprob.new_empty(floats) if floats else None
         _serving.token_logprobs(
             logits.data_ptr(), logits.stride(0), targets.data_ptr(), logprob.data_ptr(), entropy.data_ptr(),
             rank.data_ptr(), top_ids.data_ptr() if top_k else 0, top_logprobs.data_ptr() if top_k else 0,
-            work.data_ptr(), rows, vocab, top_k, dtype, at, _stream(at),
+            work.data_ptr() if floats else 0, rows, vocab, top_k, dtype, at, _stream(at),
         )
     return TokenLogprobs(logprob, entropy, rank, top_ids, top_logprobs)

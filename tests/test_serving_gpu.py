@@ -661,6 +661,38 @@ def test_token_logprobs_strides_and_offsets(serving, dtype):
     assert empty.logprob.shape == (0,) and empty.top_ids.shape == (0, 4)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("vocab,top", [(5, 5), (700, 64), (5000, 30), (20011, 60), (32761, 3)])
+def test_token_logprobs_are_the_same_among_few_rows_and_many(serving, dtype, vocab, top):
+    # few rows take one launch, many take two
+    g = gen(vocab)
+    x = torch.randn(257, vocab, generator=g, device="cuda").to(dtype)
+    x[0] = -INF
+    x[1] = 1.0
+    x[2] = torch.arange(vocab, device="cuda").to(dtype)
+    x[3] = torch.finfo(dtype).min
+    x[4, vocab // 2:] = -INF
+    x[5] = torch.round(x[5])
+    x[6, vocab // 3] = NAN
+    x[7, vocab // 3] = INF
+    t = torch.randint(0, vocab, (257,), generator=g, device="cuda")
+    t[8], t[9] = -1, vocab
+    many = serving.token_logprobs(x, t, top)
+    for a, b in zip(many, serving.token_logprobs(x[:256], t[:256], top)):
+        assert torch.equal(a[:256].nan_to_num(7e7), b.nan_to_num(7e7)) if a.is_floating_point() else torch.equal(a[:256], b)
+    check_logprobs(serving.TokenLogprobs(*(v[8:] for v in many)), x[8:], t[8:], top)
+
+
+@pytest.mark.parametrize("vocab", [65528, 65529, 65530, 65537])
+def test_token_logprobs_at_the_most_spans_of_one_launch(serving, vocab):
+    g = gen(vocab)
+    wide = torch.randn(3, vocab + 9, generator=g, device="cuda").to(FP16)
+    t = torch.randint(0, vocab, (3,), generator=g, device="cuda")
+    for at in (0, 1, 7):
+        x = wide[:, at:at + vocab]
+        check_logprobs(serving.token_logprobs(x, t, 40), x, t, 40)
+
+
 def test_token_logprobs_many_rows(serving):
     x = torch.randn(70000, 33, generator=gen(6), device="cuda").to(BF16)
     t = torch.randint(0, 33, (70000,), generator=gen(7), device="cuda")

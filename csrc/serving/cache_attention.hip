@@ -708,8 +708,11 @@ __global__ __launch_bounds__(kWaves * 64, DT <= 8 ? 2 : 1) void attention_rows_k
 
 // Joins the splits of 16 rows of a slot and head, 16 lanes a row: lane j of them
 // has split j's reference and sum (a pass for each 16 splits) and the dimensions
-// 4 j .. + 3 of each 64.
-template <typename T, int kParts>
+// 4 j .. + 3 of each 64. The loads of up to 8 splits wait together (a pass of one
+// context of 16384 tokens in 32 splits: 17 us, with two at a time 29); of two
+// splits no more are asked for, which leaves room for more rows at once (4 us of
+// 119 with chunks of up to 256 tokens).
+template <typename T, int kParts, int kBatch>
 __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
   const CacheArgs& c = a.c;
   const int lane = threadIdx.x & 63, j = lane & 15, dim = c.dim;
@@ -726,13 +729,25 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
   const int64_t step = (int64_t)a.row_tile * (dim + 2);
   const float* from = a.work + ((int64_t)slot * c.heads + h) * a.splits * step;
   const float* heads = from + (int64_t)a.row_tile * dim + 2 * i;
-  const float* mine = from + (int64_t)i * dim + j * 4;
+  const float* mine = from + (int64_t)i * dim;
   float all = -kInf, total = 0.f;
   f32x4 o[kParts] = {};
   for (int first = 0; first < p.splits; first += 16) {
     const int n = p.splits - first < 16 ? p.splits - first : 16;
     const float* at = heads + (first + (j < n ? j : 0)) * step;
     const float top = at[0], sum = at[1];
+    const float* src = mine + first * step;
+    f32x4 held[kBatch][kParts];
+    auto fetch = [&](int begin) {
+#pragma unroll
+      for (int s = 0; s < kBatch; ++s)
+        if (begin + s < n) {
+#pragma unroll
+          for (int q = 0; q < kParts; ++q)
+            held[s][q] = *reinterpret_cast<const f32x4*>(src + (begin + s) * step + (q * 64 + j * 4 < dim ? q * 64 + j * 4 : 0));
+        }
+    };
+    fetch(0);
     float best = j < n ? top : -kInf;
 #pragma unroll
     for (int x = 1; x < 16; x <<= 1) best = fmaxf(best, __shfl_xor(best, x));
@@ -746,13 +761,17 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
     all = now;
 #pragma unroll
     for (int q = 0; q < kParts; ++q) o[q] *= old;
-    const float* src = mine + first * step;
-#pragma unroll 2
-    for (int s = 0; s < n; ++s) {
-      const float w = __shfl(f, (lane & 48) + s);
+#pragma unroll 1
+    for (int begin = 0; begin < n; begin += kBatch) {
 #pragma unroll
-      for (int q = 0; q < kParts; ++q)
-        if (q * 64 + j * 4 < dim) o[q] += *reinterpret_cast<const f32x4*>(src + s * step + q * 64) * w;
+      for (int s = 0; s < kBatch; ++s) {
+        const float w = __shfl(f, (lane & 48) + begin + s);
+        if (begin + s < n) {
+#pragma unroll
+          for (int q = 0; q < kParts; ++q) o[q] += held[s][q] * w;
+        }
+      }
+      if (begin + kBatch < n) fetch(begin + kBatch);
     }
   }
   if (!live) return;
@@ -786,7 +805,8 @@ hipError_t launch(const AttentionArgs& a, hipStream_t stream) {
   }
   if (hipError_t e = hipGetLastError()) return e;
   if (a.splits > 1) {
-    join_kernel<T, DT / 4><<<dim3((unsigned)(slot_count(a) * a.c.heads * (a.row_tile / 16))), 256, 0, stream>>>(a);
+    auto kernel = a.splits == 2 ? join_kernel<T, DT / 4, 2> : join_kernel<T, DT / 4, DT <= 8 ? 8 : 4>;
+    kernel<<<dim3((unsigned)(slot_count(a) * a.c.heads * (a.row_tile / 16))), 256, 0, stream>>>(a);
   }
   return hipGetLastError();
 }

@@ -834,9 +834,15 @@ int64_t split(AttentionArgs& a, int64_t per_seq) {
   // tiles a wave at least, and a context of four or fewer is not split, since a
   // join takes 3.5 us and its launch. Where many rows share a workgroup, one
   // round will do.
-  const int64_t unit = kTile * kWaves, least = 2 * unit;
+  // Where chunks of four tiles a wave make one or two rounds of workgroups, they
+  // are taken (4 contexts of 16384, 8 heads: 31 us, with two tiles 35.5; of 9000,
+  // half a round: 27.3 and 25.9).
+  const int64_t unit = kTile * kWaves, longer = 4 * unit, round = 512;
+  const bool rounds = a.row_tile != kManyRows && work * (longest / longer) >= round &&
+                      work * ((longest + longer - 1) / longer) <= 2 * round;
+  const int64_t least = rounds ? longer : 2 * unit;
   const int64_t target = a.row_tile == kManyRows ? 768 : 2048;
-  int64_t splits = longest <= 2 * least ? 1 : target / (work > 0 ? work : 1);
+  int64_t splits = longest <= 4 * unit ? 1 : target / (work > 0 ? work : 1);
   const int64_t most = (longest + least - 1) / least;
   splits = splits < 1 ? 1 : splits > most ? most : splits;
   if (splits > 256) splits = 256;

@@ -110,7 +110,7 @@ def test_w4_matmul_of_many_tokens(serving, m, n, group, zeros):
 
 @pytest.mark.parametrize("zeros", (False, True))
 @pytest.mark.parametrize("group", (32, 64, 128))
-@pytest.mark.parametrize("tiles", (257, 520, 770, 1030, 1300, 1788, 1794, 2100))
+@pytest.mark.parametrize("tiles", (257, 520, 521, 770, 1030, 1300, 1788, 1794, 2100))
 @pytest.mark.parametrize("m", (2, 16, 29, 61))
 def test_w4_matmul_of_any_number_of_rows(serving, m, tiles, group, zeros):
     # from 1 to 8 tiles of rows a workgroup, the last of them not there or not whole

@@ -34,8 +34,10 @@
 // - Rows of tokens a power of two apart fall on the same channels of the L2. A
 //   launch before lays tokens out in the order of the loads, which pays from two
 //   tiles of tokens on (64 x 16384 x 8192: 34 with it, 44 without), but not for one
-//   (16 x 28672 x 8192: 29.5 with it, 28 without). It also takes rows that 16-byte
-//   loads do not fit.
+//   (16 x 28672 x 8192: 29.5 with it, 28 without), and not for up to 128 KB of
+//   tokens, where its launch is what a call costs (32 x 4096 x 2048: a call 12.2 with
+//   it, 8.2 without; replayed from a graph 6.7 and 7.9). It also takes rows that
+//   16-byte loads do not fit.
 // - Workgroups that read the same tokens, or rows of weights a power of two apart,
 //   at the same time wait for the same channels: they start a block of columns
 //   apart (32 x 16384 x 8192: 23.4 with the packing, 26.3 without; 16 x 32768 x
@@ -360,7 +362,8 @@ int token_tiles(int m) { return m <= 16 ? 1 : m <= 32 ? 2 : 4; }
 bool whole_loads(const W4Args& a) { return a.k % 8 == 0 && a.ldx % 8 == 0 && (uintptr_t)a.x % 16 == 0; }
 bool through_lds(const W4Args& a) { return a.m <= 16 && (int64_t)a.m * a.k <= 16384; }
 bool packs(const W4Args& a) {
-  return !through_lds(a) && (a.m > 16 || !whole_loads(a));
+  const bool small = (int64_t)a.m * a.k <= 65536 && a.k % 128 == 0;  // and no columns past the last
+  return !through_lds(a) && !(whole_loads(a) && (a.m <= 16 || small));
 }
 
 template <typename T, int MT, int NT, int G, bool kZeros, bool kX>

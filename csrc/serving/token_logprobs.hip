@@ -7,8 +7,8 @@
 // consecutive logits (one 128-byte line of 16-bit ones): no other trace of the alternatives is needed,
 // since the k best logits, by value and then by lower index, lie in the k best
 // spans by their largest and then by lower index, and in these in the k best
-// groups of 64. A second launch joins a row's spans in a fixed order and reads
-// only those groups again.
+// groups of 64. A second launch, or of few rows the same workgroup, joins a row's
+// spans in a fixed order and reads only those groups again.
 //
 // Sums are fp32 over at most 4096 values a span, 64 a lane.
 //

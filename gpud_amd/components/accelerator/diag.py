@@ -48,7 +48,7 @@ DEFAULT_GEMM_TFLOPS_FLOOR = 1000.0  # v7P asm-K-loop bf16 GEMM, ~1390-1490
 DEFAULT_GEMM_FP8_TFLOPS_FLOOR = 1400.0  # 8-phase MX-fp8 GEMM, measured ~1940
 DEFAULT_HBM_GBPS_FLOOR = 4500.0
 DEFAULT_LDS_TBPS_FLOOR = 60.0
-DEFAULT_SERVING_GBPS_FLOOR = 800.0  # a whole step, measured ~1570
+DEFAULT_SERVING_GBPS_FLOOR = 800.0  # a whole step, measured ~1720
 DEFAULT_XGMI_PAIR_GBPS_FLOOR = 30.0  # per direction, pairwise sendrecv
 
 

@@ -21,8 +21,10 @@
 // What the tokens cost beside the codes decides the rest (us, measured):
 // - Every load occupies the address path for 16 cycles, however little it
 //   fetches, as long as a load of 1 KB of codes. So scales and zero points come
-//   through LDS, and tokens too while they are under 32 KB in all: 1 x 28672 x
-//   8192 takes 24 with them in LDS, 29 without.
+//   through LDS, and the tokens of few long rows too, up to 32 KB (1 x 8192 x 8192:
+//   10.1 with them in LDS, 12.4 without). Rows are staged one after another, so more
+//   and shorter ones lose by it (4 x 16384 x 1024: 5.7 and 4.9; 16 x 4096 x 1024: 6.3
+//   and 4.3), unless 16-byte loads do not fit them: LDS saves their packing.
 // - Tokens that do not fit are read by every workgroup through the L2, which is
 //   what a compute unit's second workgroup waits for: 16 x 8192 tokens by 256
 //   tiles of rows take 12.1, by 257 to 512 tiles 20.8, but with two tiles a
@@ -360,7 +362,9 @@ __global__ __launch_bounds__(256) void pack_kernel(W4Args a, T* to, int mts, boo
 
 int token_tiles(int m) { return m <= 16 ? 1 : m <= 32 ? 2 : 4; }
 bool whole_loads(const W4Args& a) { return a.k % 8 == 0 && a.ldx % 8 == 0 && (uintptr_t)a.x % 16 == 0; }
-bool through_lds(const W4Args& a) { return a.m <= 16 && (int64_t)a.m * a.k <= 16384; }
+bool through_lds(const W4Args& a) {
+  return a.m <= 16 && (int64_t)a.m * a.k <= 16384 && (a.k >= 1024 * a.m || !whole_loads(a));
+}
 bool packs(const W4Args& a) {
   const bool small = (int64_t)a.m * a.k <= 65536 && a.k % 128 == 0;  // and no columns past the last
   return !through_lds(a) && !(whole_loads(a) && (a.m <= 16 || small));

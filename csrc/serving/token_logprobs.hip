@@ -152,10 +152,12 @@ __device__ __forceinline__ void take_span(const LogprobArgs& a, const Layout& la
   const float ref = m == -kInf ? 0.f : m;
   float sum = 0.f, weighted = 0.f;
   int above = 0;
-  if (fabsf(ref) < 1e37f) {
+  if (fabsf(ref) < 0x1p20f) {
     // u = x log2 e - m log2 e in one step. The product with m is off by a
-    // rounding, the same for all values, and comes off the sums again; what
-    // lies below -1e38 (masks, -inf) is at 0 either way.
+    // rounding, the same for all values, and comes off the sums again: `off` is
+    // half a step of 2^20 log2 e at most, 2^-4, so that 2^off is near 1. From 2^31
+    // on it passes 2^7, where 2^off leaves fp32. What lies below -1e38 (masks,
+    // -inf) is at 0 either way.
     const float shift = ref * kLog2e, off = __builtin_fmaf(ref, kLog2e, -shift);
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {

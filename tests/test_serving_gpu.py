@@ -699,6 +699,32 @@ def test_token_logprobs_many_rows(serving):
     check_logprobs(serving.token_logprobs(x, t, 2), x, t, 2)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("rows", [30, 290])
+def test_token_logprobs_of_large_magnitudes(serving, rows, dtype):
+    """Finite masks over whole spans, and rows whose largest logit is far from 0; few rows and many."""
+    g, vocab = gen(rows), 9001
+    x = torch.randn(rows, vocab, generator=g, device="cuda")
+    for i, mask in enumerate((-5e9, -1e10, -1e12, -1e20, -1e30)):
+        x[4 * i] = mask  # nothing is allowed
+        x[4 * i + 1, :4096] = mask  # a whole span
+        x[4 * i + 2, 8192:] = mask  # the last one, which is not whole
+        x[4 * i + 3] = mask
+        x[4 * i + 3, 5000] = 1.0
+    x[20, 77], x[21, 8900], x[22, 4096] = 1e10, 1e30, 9e36
+    x[23] += 0.9e6
+    x[24] += 1.1e6
+    x[25] = x[25] * 10 - 3e7
+    x[26] *= 1e10
+    x[27] *= 1e30
+    x[28] = x[28] * 1e36 - 9e36
+    x = x.to(dtype)
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    t[3:20:4] = 5000
+    t[20], t[21] = 77, 3
+    check_logprobs(serving.token_logprobs(x, t, 20), x, t, 20)
+
+
 # ---------------------------------------------------------------------------
 # together, as a program uses them
 # ---------------------------------------------------------------------------

@@ -185,8 +185,9 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
     for (int m = 0; m < 4; ++m)
 #pragma unroll
       for (int k = 0; k < KB; ++k) {
-        const uint8_t* here = from + m * 4 * dim + k * 64;
-        if (!kWhole && k * 64 + g * 16 >= dim) here = from - g * 16;  // the queries are 0 there
+        // lanes past the last dimension, where the queries are 0, read the same
+        // token's first ones: another's NaN would not stay with it
+        const uint8_t* here = from + m * 4 * dim + (kWhole || k * 64 + g * 16 < dim ? k * 64 : -g * 16);
         kr[m][k] = *reinterpret_cast<const u32x4*>(here);
       }
     const int64_t ph = (int64_t)at.pid * c.heads + h;

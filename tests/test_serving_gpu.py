@@ -545,6 +545,37 @@ def test_attention_empty_batches(serving):
     assert bool((out == 0).all()) and bool((lse == -INF).all())
 
 
+@pytest.mark.parametrize("which", ["decode", "chunk"])
+@pytest.mark.parametrize("dim,group", [(80, 4), (208, 2), (48, 1), (16, 16), (112, 20)])
+def test_attention_masked_nan_keys_of_any_dimension(serving, dim, group, which):
+    """A NaN key behind the window stays behind it, wherever it lies in its tile."""
+    window, length, count = 21, 120, 1 if which == "decode" else 5
+    batch = 40
+    lens, counts = [length + b % 3 for b in range(batch)], [count] * batch
+    cache = Cache(serving, lens, 2, dim, 16)
+    starts = starts_of(lens)
+    k, v = (torch.randn(sum(lens), 2, dim, generator=gen(i), device="cuda").to(BF16) for i in (1, 2))
+    seen = []
+    for b, n in enumerate(lens):
+        first = n - count - window  # the last position that no row sees
+        at = first - b // 2 if b < 36 else first + 1 + b % 4
+        k[starts[b] + at, :, b % 16] = NAN
+        if b >= 36:
+            seen.append(b)
+    serving.cache_append(k, v, *cache.tensors, cache.table, ints(lens), ints(starts))
+    rows = starts_of(counts)
+    q = torch.randn(rows[-1], 2 * group, dim, generator=gen(3), device="cuda").to(BF16)
+    out, lse = serving.cache_attention(
+        q, *cache.tensors, cache.table, ints(lens), None if count == 1 else ints(rows), window=window
+    )
+    check_attention(cache, q, lens, rows, (out, lse), window=window, skip=seen)
+    for b in seen:
+        for i in range(count):
+            pos = lens[b] - count + i
+            sees = lens[b] - count - window + 1 + b % 4 > pos - window
+            assert bool(torch.isnan(out[rows[b] + i]).all()) == sees and bool(torch.isnan(lse[rows[b] + i]).all()) == sees
+
+
 # ---------------------------------------------------------------------------
 # token_logprobs
 # ---------------------------------------------------------------------------

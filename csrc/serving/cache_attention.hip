@@ -385,7 +385,7 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
           f32x4 o = part[0][d][lane];
 #pragma unroll
           for (int w = 1; w < kWaves; ++w) o += part[w][d][lane];
-          if (kWhole || d * 16 < dim) store4(out + d * 16, o * inv);
+          if ((kWhole || d * 16 < dim) && !p.keep) store4(out + d * 16, o * inv);
         }
         if (wave == 0 && g == 0)
           a.lse[(int64_t)(p.row0 + tok) * a.q_heads + head] = (all + __builtin_amdgcn_logf(total)) * kLn2;
@@ -691,7 +691,7 @@ __global__ __launch_bounds__(kWaves * 64, DT <= 8 ? 2 : 1) void attention_rows_k
       T* out = (T*)a.out + (int64_t)(p.row0 + tok) * a.o_row + head * a.o_head + g * 4;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
-        if (kWhole || d * 16 < dim) store4(out + d * 16, acc[t][d] * inv);
+        if ((kWhole || d * 16 < dim) && !p.keep) store4(out + d * 16, acc[t][d] * inv);
       if (g == 0) a.lse[(int64_t)(p.row0 + tok) * a.q_heads + head] = (top[t] + __builtin_amdgcn_logf(sum[t])) * kLn2;
     } else {
       float* to = a.work + (((int64_t)slot * c.heads + h) * a.splits + split) * a.row_tile * (dim + 2);
@@ -867,7 +867,7 @@ AttentionPlan plan_attention(const AttentionArgs& all) {
     a.few = few;
     a.many = many;
     a.per = per;
-    a.fill_tail = all.fill_tail && per == 0;
+    a.tail = per == 0 ? all.tail : kLeaveTail;
     a.work = all.work ? all.work + plan.floats : nullptr;
     plan.floats += split(a, per_seq);
   };

@@ -46,6 +46,7 @@ struct Place {
   int first, last;          // positions of the first and the last of them
   int lo, hi, splits;       // tokens seen: [lo, hi); workgroups with any
   bool broken;              // longer than its row of the table: its results are NaN
+  bool keep;                // rows behind the last sequence whose output stays as it was
 };
 
 // Rows of a tile are a power of two.
@@ -118,7 +119,8 @@ __host__ __device__ inline bool place_of_slot(const AttentionArgs& a, int group,
   }
   if (!rows_of(c, p)) return false;
   if ((int64_t)p.tile * a.row_tile >= (int64_t)p.count * group) return false;
-  if (p.b == c.batch ? !a.fill_tail : !takes(a, group, p.count)) return false;
+  if (p.b == c.batch ? a.tail == kLeaveTail : !takes(a, group, p.count)) return false;
+  p.keep = p.b == c.batch && a.tail == kTailLse;
   fill_place(a, group, p);
   return true;
 }

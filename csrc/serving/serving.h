@@ -55,6 +55,10 @@ struct AppendArgs {
 };
 hipError_t launch_cache_append(const AppendArgs& a, hipStream_t stream);
 
+// Rows behind the last sequence: left alone; their lse becomes -inf; their
+// output becomes 0 as well.
+enum Tail : int { kLeaveTail = 0, kTailLse = 1, kFillTail = 2 };
+
 struct AttentionArgs {
   CacheArgs c;
   const void* q;          // [rows][q_heads][dim], last dimension dense
@@ -63,7 +67,7 @@ struct AttentionArgs {
   float* work;            // plan_attention() floats, or null if 0
   int64_t q_row, q_head, o_row, o_head;
   int q_heads, window;    // window 0: none
-  int fill_tail;          // rows behind the last sequence become 0 / -inf
+  int tail;               // a Tail: what becomes of rows behind the last sequence
   float scale;
   int dtype;
   int64_t longest;        // longest sequence as far as known: steers the split

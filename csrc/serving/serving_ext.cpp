@@ -199,7 +199,7 @@ PyObject* cache_attention(PyObject*, PyObject* const* args, Py_ssize_t count) {
     a.q_heads = n.small();
     a.window = n.small();
     a.longest = n.whole();
-    a.fill_tail = n.small();
+    a.tail = n.small() ? kFillTail : kTailLse;
     a.scale = (float)n.real();
     a.dtype = n.small();
     OnDevice on(n.small());
@@ -270,7 +270,7 @@ std::vector<std::vector<int64_t>> attention_places(const std::vector<int32_t>& s
   all.c.dim = 128;
   all.q_heads = q_heads;
   all.window = window;
-  all.fill_tail = fill_tail;
+  all.tail = fill_tail ? kFillTail : kLeaveTail;
   all.longest = max_seq_len;
   const int group = q_heads / heads;
   std::vector<std::vector<int64_t>> got;

@@ -576,6 +576,23 @@ def test_attention_masked_nan_keys_of_any_dimension(serving, dim, group, which):
             assert bool(torch.isnan(out[rows[b] + i]).all()) == sees and bool(torch.isnan(lse[rows[b] + i]).all()) == sees
 
 
+@pytest.mark.parametrize("counts", [[3, 2], [3, 200], [100], [1, 1]])
+def test_attention_lse_of_rows_behind_the_last(serving, counts):
+    """With `out` given they keep what it held, and their lse is -inf as without it."""
+    lens = [n + 30 for n in counts]
+    for dim in (64, 208):
+        cache, _, _ = filled(serving, lens, 2, dim, 16)
+        starts = starts_of(counts)
+        q = torch.randn(starts[-1] + 70, 8, dim, generator=gen(5), device="cuda").to(BF16)
+        mine = torch.full_like(q, 5.0)
+        for _ in range(3):
+            before = torch.full((q.shape[0], 8), 7.0, device="cuda")  # what the next tensor of this size is made of
+            del before
+            _, lse = serving.cache_attention(q, *cache.tensors, cache.table, ints(lens), ints(starts), out=mine)
+            check_attention(cache, q, lens, starts, (mine, lse))
+            assert bool((mine[starts[-1]:] == 5).all()) and bool((lse[starts[-1]:] == -INF).all())
+
+
 # ---------------------------------------------------------------------------
 # token_logprobs
 # ---------------------------------------------------------------------------

@@ -85,7 +85,8 @@ __device__ __forceinline__ void store4(T* to, f32x4 v) {
 
 // How a lane's 16 tokens, all of one page, weigh in: a score's power of two is
 // unit q . K + log, with the value's scale in it, and `back` takes that out of
-// the sum again.
+// the sum again. The scale of a page that no row sees (not `within`) is left out:
+// it may be anything, and a score of -inf would not keep it from the sum.
 struct Weighing {
   float unit, log, back;
   __device__ __forceinline__ Weighing(bool known, bool within, float ks, float vs, float scale) {
@@ -223,7 +224,7 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
     for (; base < end; base += kWaves * kTile) {
       const int tok0 = base + g * 16;  // the lane's 16 tokens for P and V
       load_values(base, here);
-      Weighing by(here.known, tok0 < end, ks, vs, a.scale);
+      Weighing by(here.known, tok0 < end && tok0 + 16 > p.lo, ks, vs, a.scale);
 
       f32x4 s[QT][4] = {};
 #pragma unroll
@@ -559,7 +560,7 @@ __global__ __launch_bounds__(kWaves * 64, DT <= 8 ? 2 : 1) void attention_rows_k
 
         if (base <= w_last && base + kTile - 1 > w_low) {
           const int tok0 = base + g * 16;
-          Weighing by(known, tok0 < end, ks, vs, a.scale);
+          Weighing by(known, tok0 < end && tok0 + 16 > p.lo, ks, vs, a.scale);
           f32x4 s[QT][4] = {};
 #pragma unroll
           for (int m = 0; m < 4; ++m)

@@ -401,8 +401,8 @@ def cache_attention(
 
     Returns (out [T, q_heads, dim] in q's type, lse float32 [T, q_heads]), lse
     the logarithm of the sum of the exponentials of a row's scores. The scales
-    of pages that are read have to be positive and finite. A row that
-    sees nothing gets 0 and -inf. A sequence whose pages are out of range, or
+    of pages that a row sees have to be positive and finite; others may hold
+    anything. A row that sees nothing gets 0 and -inf. A sequence whose pages are out of range, or
     that is longer than its row of ``block_table``, gets NaN. Rows behind the
     last sequence are left as they were in ``out`` if that is given, and else
     0; their lse is -inf. ``out`` may not share memory with the other arguments.

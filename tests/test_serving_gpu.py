@@ -593,6 +593,28 @@ def test_attention_lse_of_rows_behind_the_last(serving, counts):
             assert bool((mine[starts[-1]:] == 5).all()) and bool((lse[starts[-1]:] == -INF).all())
 
 
+@pytest.mark.parametrize("value", [0.0, -1.0, INF, NAN])
+@pytest.mark.parametrize("dim,count", [(64, 1), (64, 5), (128, 100), (80, 3), (80, 90), (208, 2)])
+def test_attention_scales_of_pages_that_no_row_sees(serving, dim, count, value):
+    """Pages behind the window and behind the last token hold whatever a program left there."""
+    window, lens, counts = 10, [190, 60 + count], [count, count]
+    cache, _, _ = filled(serving, lens, 2, dim, 16, blocks=13)
+    table = cache.table
+    spare = set(range(cache.tensors[0].shape[0])) - set(table.flatten().tolist())
+    table[table < 0] = spare.pop()  # a page that nothing was written to
+    _, _, ks, vs = cache.tensors
+    kept = [t.clone() for t in (ks, vs)]
+    for b, n in enumerate(lens):
+        for block in range(13):
+            if block * 16 + 15 <= n - count - window or block * 16 >= n:
+                ks[int(table[b, block])] = vs[int(table[b, block])] = value
+    starts = starts_of(counts)
+    q = torch.randn(starts[-1], 8, dim, generator=gen(3), device="cuda").to(BF16)
+    got = serving.cache_attention(q, *cache.tensors, table, ints(lens), None if count == 1 else ints(starts), window=window)
+    ks.copy_(kept[0]), vs.copy_(kept[1])
+    check_attention(cache, q, lens, starts, got, window=window)
+
+
 # ---------------------------------------------------------------------------
 # token_logprobs
 # ---------------------------------------------------------------------------

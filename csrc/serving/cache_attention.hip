@@ -17,8 +17,9 @@
 //
 // Codes become q's type for the scores and fp16 for the values: both hold e4m3
 // exactly. The weights are rounded to fp16 (2^-11; bf16 would show in bf16
-// results): they are p vs over the largest p vs so far, so at most 1, and what
-// falls under fp16's range is under 2^-24 of the result. Sums are fp32.
+// results). They are p vs over a reference that follows the largest p vs so far,
+// so that weights down to 2^-21 of it keep their 11 bits: a context may be
+// shared by a million tokens beside a single large one. Sums are fp32.
 //
 // Of few rows, a workgroup's 4 waves take turns at tiles of 64 tokens and join
 // in LDS; of many, they have rows of their own and share the tiles. Long
@@ -96,6 +97,14 @@ struct Weighing {
     back = 1.f / v;
   }
 };
+
+// What weights are relative to, in powers of two: 2^7 under the largest so far
+// when it moves, and it moves only where a weight would pass 2^15. So the largest
+// weights fill fp16's range (65504), and those with 11 bits reach down to 2^-21 of
+// the largest, with fewer bits to 2^-31.
+__device__ __forceinline__ float reference(float top, float best) {
+  return best > top + 15.f ? best - 7.f : top;
+}
 
 // Codes that one workgroup reads once pass by the L2.
 template <int QT>
@@ -268,9 +277,7 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(DT, QT)) void attention_kerne
         best = __builtin_fmaf(best, by.unit, by.log);
         best = fmaxf(best, __shfl_xor(best, 16));
         best = fmaxf(best, __shfl_xor(best, 32));
-        // the reference moves only where weights would leave 2^8: fp16 and fp32
-        // hold them as exactly there
-        const float now = best > top[t] + 8.f ? best : top[t];
+        const float now = reference(top[t], best);
         if (__any(now != top[t])) {
           const float f = now == -kInf ? 0.f : __builtin_amdgcn_exp2f(top[t] - now);
           sum[t] *= f;
@@ -594,9 +601,7 @@ __global__ __launch_bounds__(kWaves * 64, DT <= 8 ? 2 : 1) void attention_rows_k
             best = __builtin_fmaf(best, by.unit, by.log);
             best = fmaxf(best, __shfl_xor(best, 16));
             best = fmaxf(best, __shfl_xor(best, 32));
-            // the reference moves only where weights would leave 2^8: fp16 and fp32
-            // hold them as exactly there
-            const float now = best > top[t] + 8.f ? best : top[t];
+            const float now = reference(top[t], best);
             if (__any(now != top[t])) {
               const float f = now == -kInf ? 0.f : __builtin_amdgcn_exp2f(top[t] - now);
               sum[t] *= f;

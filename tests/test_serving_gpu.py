@@ -615,6 +615,34 @@ def test_attention_scales_of_pages_that_no_row_sees(serving, dim, count, value):
     check_attention(cache, q, lens, starts, got, window=window)
 
 
+@pytest.mark.parametrize("rows", [1, 100])
+def test_attention_of_many_small_weights_beside_a_large_one(serving, rows):
+    """One token with half of the weight, and 1.6 million others that share the rest."""
+    length, dim, page = 1605000, 64, 4096
+    cache = Cache(serving, [length], 1, dim, page, spare=0)
+    k, v = torch.zeros(length, 1, dim, dtype=FP16, device="cuda"), torch.ones(length, 1, dim, dtype=FP16, device="cuda")
+    k[0, 0, 0] = 14.0
+    v[0] = -0.25
+    serving.cache_append(k, v, *cache.tensors, cache.table, ints([length]), ints([0, length]))
+    q = torch.zeros(rows, 1, dim, dtype=FP16, device="cuda")
+    q[:, :, 0] = math.log(length) / 14
+    for longest in (1, None):
+        out, lse = serving.cache_attention(
+            q, *cache.tensors, cache.table, ints([length]), ints([0, rows]), scale=1.0, max_seq_len=longest
+        )
+        pos = torch.arange(length - rows, length, device="cuda", dtype=torch.float64)[:, None]
+        sink = torch.exp(q[:, 0, :1].double() * 14)
+        want = (pos - 0.25 * sink) / (pos + sink)
+        # fp16 weights, 2^-11 of each; fp32 sums, of a product 2 terms and of the weights
+        # one a tile of 64 tokens; the score's fp32 sum and power
+        mass = (pos + 0.25 * sink) / (pos + sink)
+        rel = (length / 64 + 64 + 14.3 * 2 * (dim + 8)) * E32
+        bound = float((mass * (2.0**-11 + 2 * rel) + want.abs() * rel).max()) + half_step(FP16)
+        print(float((out[:, 0].double() - want).abs().max()), bound)
+        assert float((out[:, 0].double() - want).abs().max()) <= bound
+        close(lse, torch.log(pos + sink), rel + 16 * 4 * E32)
+
+
 # ---------------------------------------------------------------------------
 # token_logprobs
 # ---------------------------------------------------------------------------

@@ -12,7 +12,9 @@
 // zero point, where all are 8) off again inside the fp32 accumulator; it is one
 // for all weight rows and gives the sum of x that zero points are times. Each
 // product is of x with a whole number of at most 5 bits, and nothing is rounded
-// before the fp32 sum of a group, which its scale multiplies.
+// before the fp32 sum of a group, which its scale multiplies. On its way the sum
+// of 128 columns comes to 24 128 + 31 32 = 2^12 times the largest x, whatever its
+// result, so x has to be under 2^115 for it to stay within fp32.
 //
 // The 8 waves of a workgroup split the columns and join their sums in LDS, in
 // the waves' order, so that results do not depend on timing. 16 waves are slower

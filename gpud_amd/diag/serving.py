@@ -195,7 +195,9 @@ def w4_matmul(
     M up to 64; larger M, up to ``MAX_TOKENS``, are taken 64 rows at a time.
     K is at most ``MAX_COLUMNS``, N 2^26 and M N 2^33. ``out`` may not share
     memory with the other arguments.
-    Sums are fp32, rounded once to x's type. ``x`` has to be finite, and under 1e37 in magnitude.
+    Sums are fp32, rounded once to x's type. ``x`` has to be finite, and under
+    2^115 (4e34) in magnitude: a group's sum is formed from x times whole numbers
+    up to 31 and comes to 2^12 times the largest x on its way.
     """
     dtype = _primary("x", x, 2, _HALVES)
     m, k = x.shape

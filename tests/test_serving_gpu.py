@@ -158,6 +158,32 @@ def test_w4_matmul_large_values_and_zero_rows(serving):
     assert bool(torch.isnan(got[2]).all()) and not bool(torch.isnan(got[[0, 1, 3]]).any())
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m", [1, 16, 20, 50])
+def test_w4_matmul_of_the_largest_values(serving, m, group, zeros):
+    """Values just under 2^115 of one sign: the sums of a group stay within fp32."""
+    n, k = 40, 500
+    x = torch.full((m, k), 2.0**115, dtype=torch.float64, device="cuda").to(BF16)
+    x = (x.double() * (1 - 2.0**-8)).to(BF16)
+    x[m // 2] *= -1
+    codes = torch.randint(0, 16, (n, k), generator=gen(m), device="cuda")
+    codes[1] = torch.arange(k, device="cuda") % 2 * 2 + 7
+    codes[2], codes[3] = 0, 15
+    groups = -(-k // group)
+    scales = torch.full((n, groups), 2.0**-6, dtype=BF16, device="cuda")
+    z = torch.full((n, groups), 8, device="cuda")
+    if zeros:
+        z[4], z[5] = 0, 15
+    packed = serving.pack_w4(codes, scales, z if zeros else None, group_size=group)
+    zz = z.double()[:, torch.arange(k, device="cuda") // group]
+    want = x.double() @ ((codes.double() - zz) / 64).t()
+    size = x.double().abs() @ ((codes.double() + 32 + zz) / 64).t()
+    bound = half_step(BF16) * want.abs() + (2 * group + groups + 16) * E32 * size
+    got = serving.w4_matmul(x, *packed, out_features=n, group_size=group)
+    close(got, want, bound * (1 + half_step(BF16)))
+
+
 # ---------------------------------------------------------------------------
 # cache
 # ---------------------------------------------------------------------------

@@ -65,8 +65,16 @@ class Numbers {
     return v;
   }
   int small() { return (int)whole(); }
+  // of a tensor that may be missing
   template <typename T = void>
   T* pointer() { return ptr<T>((uintptr_t)whole()); }
+  // of one that has to be there: a tensor may have a shape and no memory
+  template <typename T = void>
+  T* memory() {
+    T* p = pointer<T>();
+    if (!p) throw std::domain_error("a tensor has no memory");
+    return p;
+  }
   double real() {
     const double v = PyFloat_AsDouble(args_[at_++]);
     if (v == -1 && PyErr_Occurred()) throw py::error_already_set();
@@ -86,6 +94,8 @@ PyObject* guarded(F f) {
     e.restore();
   } catch (const std::invalid_argument& e) {
     PyErr_SetString(PyExc_TypeError, e.what());
+  } catch (const std::domain_error& e) {
+    PyErr_SetString(PyExc_ValueError, e.what());
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
   }
@@ -95,7 +105,7 @@ PyObject* none() { Py_RETURN_NONE; }
 
 W4Args w4_args(Numbers& n) {
   W4Args a{};
-  a.x = n.pointer();
+  a.x = n.memory();
   a.ldx = n.whole();
   a.m = n.small();
   a.n = n.small();
@@ -116,12 +126,12 @@ PyObject* w4_matmul(PyObject*, PyObject* const* args, Py_ssize_t count) {
   return guarded([&] {
     Numbers n(args, count, 15);
     W4Args a = w4_args(n);
-    a.codes = n.pointer<uint8_t>();
-    a.scales = n.pointer();
+    a.codes = n.memory<uint8_t>();
+    a.scales = n.memory();
     a.zeros = n.pointer<uint8_t>();
-    a.y = n.pointer();
+    a.y = n.memory();
     a.ldy = n.whole();
-    a.work = n.pointer();
+    a.work = w4_workspace(a) ? n.memory() : n.pointer();
     OnDevice on(n.small());
     OnDevice::check(launch_w4_matmul(a, stream_of(n.whole())), "w4_matmul");
     return none();
@@ -130,12 +140,12 @@ PyObject* w4_matmul(PyObject*, PyObject* const* args, Py_ssize_t count) {
 
 CacheArgs cache_args(Numbers& n) {
   CacheArgs c{};
-  c.k = n.pointer<uint8_t>();
-  c.v = n.pointer<uint8_t>();
-  c.k_scale = n.pointer<float>();
-  c.v_scale = n.pointer<float>();
+  c.k = n.memory<uint8_t>();
+  c.v = n.memory<uint8_t>();
+  c.k_scale = n.memory<float>();
+  c.v_scale = n.memory<float>();
   c.table = n.pointer<int32_t>();
-  c.lens = n.pointer<int32_t>();
+  c.lens = n.memory<int32_t>();
   c.starts = n.pointer<int32_t>();
   c.ldt = n.whole();
   c.pages = n.small();
@@ -145,6 +155,7 @@ CacheArgs cache_args(Numbers& n) {
   c.batch = n.small();
   c.blocks = n.small();
   c.rows = n.small();
+  if (c.blocks && !c.table) throw std::domain_error("block_table has no memory");
   return c;
 }
 
@@ -153,10 +164,10 @@ PyObject* cache_append(PyObject*, PyObject* const* args, Py_ssize_t count) {
     Numbers n(args, count, 24);
     AppendArgs a{};
     a.c = cache_args(n);
-    a.k_new = n.pointer();
+    a.k_new = n.memory();
     a.k_row = n.whole();
     a.k_head = n.whole();
-    a.v_new = n.pointer();
+    a.v_new = n.memory();
     a.v_row = n.whole();
     a.v_head = n.whole();
     a.dtype = n.small();
@@ -188,13 +199,13 @@ PyObject* cache_attention(PyObject*, PyObject* const* args, Py_ssize_t count) {
     Numbers n(args, count, 31);
     AttentionArgs a{};
     a.c = cache_args(n);
-    a.q = n.pointer();
+    a.q = n.memory();
     a.q_row = n.whole();
     a.q_head = n.whole();
-    a.out = n.pointer();
+    a.out = n.memory();
     a.o_row = n.whole();
     a.o_head = n.whole();
-    a.lse = n.pointer<float>();
+    a.lse = n.memory<float>();
     a.work = n.pointer<float>();
     a.q_heads = n.small();
     a.window = n.small();
@@ -202,6 +213,7 @@ PyObject* cache_attention(PyObject*, PyObject* const* args, Py_ssize_t count) {
     a.tail = n.small() ? kFillTail : kTailLse;
     a.scale = (float)n.real();
     a.dtype = n.small();
+    if (!a.work && plan_attention(a).floats) throw std::domain_error("the workspace has no memory");
     OnDevice on(n.small());
     OnDevice::check(launch_cache_attention(a, stream_of(n.whole())), "cache_attention");
     return none();
@@ -221,12 +233,12 @@ PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t count) {
   return guarded([&] {
     Numbers n(args, count, 15);
     LogprobArgs a{};
-    a.logits = n.pointer();
+    a.logits = n.memory();
     a.ld = n.whole();
-    a.targets = n.pointer<int64_t>();
-    a.logprob = n.pointer<float>();
-    a.entropy = n.pointer<float>();
-    a.rank = n.pointer<int64_t>();
+    a.targets = n.memory<int64_t>();
+    a.logprob = n.memory<float>();
+    a.entropy = n.memory<float>();
+    a.rank = n.memory<int64_t>();
     a.top_ids = n.pointer<int64_t>();
     a.top_logprobs = n.pointer<float>();
     a.work = n.pointer<float>();
@@ -234,6 +246,8 @@ PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t count) {
     a.vocab = n.small();
     a.top = n.small();
     a.dtype = n.small();
+    if ((a.top && !(a.top_ids && a.top_logprobs)) || (!a.work && logprob_workspace(a.rows, a.vocab, a.dtype)))
+      throw std::domain_error("a tensor has no memory");
     OnDevice on(n.small());
     OnDevice::check(launch_token_logprobs(a, stream_of(n.whole())), "token_logprobs");
     return none();

@@ -18,8 +18,9 @@ captured into a graph: workspaces are allocated per call from torch's
 allocator, so two graphs share none. Arguments that do not fit raise
 ``TypeError`` or ``ValueError`` before anything is enqueued. Page numbers,
 lengths and tokens that live on the GPU are bounded there: see each function.
-The operators have no backward pass and refuse inputs that require a gradient
-while gradients are recorded.
+Tensors that have a shape but no memory (freed storages, fake tensors, wrapper
+subclasses) are among those. The operators have no backward pass and refuse
+inputs that require a gradient while gradients are recorded.
 """
 
 from __future__ import annotations
@@ -102,6 +103,14 @@ def _check_input(name: str, t: torch.Tensor, device: Optional[torch.device], dty
 def _check_gpu(device: torch.device) -> None:
     if device.type != "cuda":
         raise ValueError(f"the tensors must be on a GPU, not on {device}")
+
+
+def _memory(name: str, t: torch.Tensor) -> int:
+    """The address of a tensor that may be missing: 0 has to mean that it is."""
+    at = t.data_ptr()
+    if not at:
+        raise ValueError(f"{name} has no memory")
+    return at
 
 
 def _check_shape(name: str, t: torch.Tensor, shape: Tuple[int, ...]) -> None:
@@ -217,7 +226,8 @@ def w4_matmul(
     if zeros is not None and not _fits(zeros, at, torch.uint8, (tiles, groups, 16)):
         _check_input("zeros", zeros, device, (torch.uint8,), 3)
         _check_shape("zeros", zeros, (tiles, groups, 16))
-    if codes.data_ptr() % 16 or scales.data_ptr() % 8 or (zeros is not None and zeros.data_ptr() % 4):
+    zp = 0 if zeros is None else _memory("zeros", zeros)
+    if codes.data_ptr() % 16 or scales.data_ptr() % 8 or zp % 4:
         raise ValueError("codes, scales and zeros must be aligned to 16, 8 and 4 bytes")
     if out is None:
         _check_gpu(device)
@@ -236,7 +246,7 @@ def w4_matmul(
         size = _serving.w4_workspace(*args)
         work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         _serving.w4_matmul(
-            *args, codes.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(),
+            *args, codes.data_ptr(), scales.data_ptr(), zp,
             out.data_ptr(), out.stride(0), work.data_ptr() if size else 0, at, _stream(at),
         )
     return out
@@ -318,7 +328,7 @@ def _cache_args(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query
         if not _fits(query_start, at, torch.int32, (batch + 1,)):
             _check_input("query_start", query_start, device, (torch.int32,), 1)
             _check_shape("query_start", query_start, (batch + 1,))
-        starts = query_start.data_ptr()
+        starts = _memory("query_start", query_start)
     kp, vp = k_cache.data_ptr(), v_cache.data_ptr()
     if kp % 16 or vp % 16:
         raise ValueError("k_cache and v_cache must be aligned to 16 bytes")

@@ -338,6 +338,60 @@ def test_new_cache_refuses_sizes():
             serving.new_cache(*bad, device="cpu")
 
 
+W4 = [64, 256, 3, 20, 256, 128, 0, 64, 64, 0, 64, 20, 0, 0, 0]
+CACHE = [64, 64, 64, 64, 64, 64, 0, 4, 5, 2, 16, 64, 3, 4, 3]
+APPEND = CACHE + [64, 128, 64, 64, 128, 64, 0, 0, 0]
+ATTENTION = CACHE + [64, 256, 64, 64, 256, 64, 64, 0, 4, 0, 64, 1, 0.125, 0, 0, 0]
+LOGPROBS = [64, 9, 64, 64, 64, 64, 64, 64, 0, 2, 9, 3, 0, 0, 0]
+
+
+@pytest.mark.parametrize(
+    "name,args,at",
+    [("w4_matmul", W4, i) for i in (0, 7, 8, 10)]
+    + [("cache_append", APPEND, i) for i in (0, 1, 2, 3, 4, 5, 15, 18)]
+    + [("cache_attention", ATTENTION, i) for i in (0, 1, 2, 3, 4, 5, 15, 18, 21)]
+    + [("token_logprobs", LOGPROBS, i) for i in (0, 2, 3, 4, 5, 6, 7)],
+)
+def test_tensors_without_memory_are_refused_before_a_launch(name, args, at):
+    args = list(args)
+    args[at] = 0
+    with pytest.raises(ValueError, match="no memory"):
+        getattr(_serving, name)(*args)
+
+
+def test_workspaces_without_memory_are_refused_before_a_launch():
+    w4 = [64, 1024, 64, 4096, 1024, 128, 0]
+    assert _serving.w4_workspace(*w4) == 0
+    w4[1:3] = [2048, 64]
+    w4[4] = 2048
+    assert _serving.w4_workspace(*w4) > 0
+    with pytest.raises(ValueError, match="no memory"):
+        _serving.w4_matmul(*w4, 64, 64, 0, 64, 4096, 0, 0, 0)
+    assert _serving.attention_workspace(1, 1, 8, 32, 128, 0, 0, 100000) > 0
+    long = [64, 64, 64, 64, 64, 64, 0, 1600, 1600, 8, 64, 128, 1, 1600, 1]
+    with pytest.raises(ValueError, match="no memory"):
+        _serving.cache_attention(*long, 64, 4096, 128, 64, 4096, 128, 64, 0, 32, 0, 100000, 1, 0.1, 0, 0, 0)
+    assert _serving.logprob_workspace(300, 32000, 0) > 0
+    with pytest.raises(ValueError, match="no memory"):
+        _serving.token_logprobs(64, 32000, 64, 64, 64, 64, 0, 0, 0, 300, 32000, 0, 0, 0, 0)
+
+
+def test_missing_and_empty_tensors_are_told_apart():
+    """Zero points and starts may be missing; given without memory they are not that."""
+    gone = torch.zeros(2, 2, 16, dtype=torch.uint8)
+    gone.untyped_storage().resize_(0)
+    a = w4_args(zeros=gone)
+    with pytest.raises(ValueError, match="zeros has no memory"):
+        serving.w4_matmul(a.pop("x"), a.pop("codes"), a.pop("scales"), a.pop("zeros"), **a)
+    starts = torch.zeros(4, dtype=torch.int32)
+    starts.untyped_storage().resize_(0)
+    k = torch.zeros(3, 2, 64, dtype=BF16)
+    with pytest.raises(ValueError, match="query_start has no memory"):
+        serving.cache_append(k, k, **cache_args(query_start=starts))
+    with pytest.raises(ValueError, match="query_start has no memory"):
+        serving.cache_attention(torch.zeros(3, 4, 64, dtype=BF16), **cache_args(query_start=starts))
+
+
 # -- the diagnostic that runs them -------------------------------------------
 
 

@@ -946,6 +946,31 @@ def test_step_in_two_graphs_and_on_another_stream(serving):
     assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
 
 
+def test_tensors_without_memory_are_refused(serving):
+    """Freed storages, in place of each tensor of each call."""
+
+    def each(call, *tensors):
+        call(*tensors)
+        for i, t in enumerate(tensors):
+            gone = torch.empty_like(t)
+            gone.untyped_storage().resize_(0)
+            with pytest.raises(ValueError, match="no memory"):
+                call(*tensors[:i], gone, *tensors[i + 1:])
+
+    x, (codes, scales, z), _, _ = w4_case(serving, 40, 48, 1100, 64, True, BF16)
+    out = x.new_empty(40, 48)
+    each(lambda x, c, s, z, o: serving.w4_matmul(x, c, s, z, out_features=48, group_size=64, out=o), x, codes, scales, z, out)
+    cache, k, v = filled(serving, [40, 70], 2, 64, 16)
+    lens, starts = ints([40, 70]), ints([0, 40, 110])
+    each(serving.cache_append, k, v, *cache.tensors, cache.table, lens, starts)
+    each(serving.cache_append, k[:2], v[:2], *cache.tensors, cache.table, lens)
+    q = torch.randn(110, 4, 64, device="cuda").to(BF16)
+    each(lambda *t: serving.cache_attention(*t[:-1], out=t[-1]), q, *cache.tensors, cache.table, lens, starts, q.clone())
+    logits, targets = torch.randn(300, 100, device="cuda"), torch.zeros(300, dtype=torch.long, device="cuda")
+    each(lambda x, t: serving.token_logprobs(x, t, 3), logits, targets)
+    torch.cuda.synchronize()
+
+
 def test_inference_without_gradients_and_with(serving):
     x, (codes, scales, z), want, bound = w4_case(serving, 2, 16, 128, 128, False, BF16)
     x.requires_grad_()

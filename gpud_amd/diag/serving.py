@@ -19,8 +19,9 @@ allocator, so two graphs share none. Arguments that do not fit raise
 ``TypeError`` or ``ValueError`` before anything is enqueued. Page numbers,
 lengths and tokens that live on the GPU are bounded there: see each function.
 Tensors that have a shape but no memory (freed storages, fake tensors, wrapper
-subclasses) are among those. The operators have no backward pass and refuse
-inputs that require a gradient while gradients are recorded.
+subclasses) are among those. The operators have no backward pass and no forward
+mode: they refuse inputs that require a gradient while gradients are recorded,
+and inputs with a tangent.
 """
 
 from __future__ import annotations
@@ -29,6 +30,7 @@ import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _serving
 
@@ -103,6 +105,13 @@ def _check_input(name: str, t: torch.Tensor, device: Optional[torch.device], dty
 def _check_gpu(device: torch.device) -> None:
     if device.type != "cuda":
         raise ValueError(f"the tensors must be on a GPU, not on {device}")
+
+
+def _refuse_tangents(**tensors) -> None:
+    """Forward mode marks a tensor by its tangent alone; it would be dropped without a word."""
+    for name, t in tensors.items():
+        if isinstance(t, torch.Tensor) and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name} has a tangent, and the operator has no forward mode")
 
 
 def _memory(name: str, t: torch.Tensor) -> int:
@@ -208,6 +217,8 @@ def w4_matmul(
     2^115 (4e34) in magnitude: a group's sum is formed from x times whole numbers
     up to 31 and comes to 2^12 times the largest x on its way.
     """
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x=x, scales=scales, out=out)
     dtype = _primary("x", x, 2, _HALVES)
     m, k = x.shape
     n = int(out_features)
@@ -365,6 +376,8 @@ def cache_append(
     out of range, or whose position is negative, are left out. A page that gets
     tokens may stand in the table once only.
     """
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(k=k, v=v, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
     dtype = _primary("k", k, 3, _HALVES)
     device, at = k.device, k.get_device()
     _check_input("v", v, device, (k.dtype,), 3)
@@ -419,6 +432,8 @@ def cache_attention(
     last sequence are left as they were in ``out`` if that is given, and else
     0; their lse is -inf. ``out`` may not share memory with the other arguments.
     """
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(q=q, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, out=out)
     dtype = _primary("q", q, 3, _HALVES)
     device, at = q.device, q.get_device()
     rows, q_heads, dim = q.shape
@@ -498,6 +513,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
     row with NaN or +inf has NaN as its log probability and entropy; NaN comes
     first among its alternatives.
     """
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(logits=logits)
     dtype = _primary("logits", logits, 2, _DTYPES)
     device, at = logits.device, logits.get_device()
     rows, vocab = logits.shape

@@ -392,6 +392,39 @@ def test_missing_and_empty_tensors_are_told_apart():
         serving.cache_attention(torch.zeros(3, 4, 64, dtype=BF16), **cache_args(query_start=starts))
 
 
+def test_tangents_are_refused():
+    """In forward mode, and under torch.func.jvp, whose tensors require no gradient either."""
+
+    def w4(**change):
+        a = w4_args(**change)
+        return serving.w4_matmul(a.pop("x"), a.pop("codes"), a.pop("scales"), a.pop("zeros"), **a)
+
+    half = torch.zeros(3, 2, 64, dtype=BF16)
+    calls = [
+        (lambda t: w4(x=t), torch.zeros(3, 256, dtype=BF16)),
+        (lambda t: w4(scales=t), torch.zeros(2, 2, 16, dtype=BF16)),
+        (lambda t: w4(out=t), torch.zeros(3, 20, dtype=BF16)),
+        (lambda t: serving.cache_append(t, half, **cache_args()), half),
+        (lambda t: serving.cache_append(half, t, **cache_args()), half),
+        (lambda t: serving.cache_append(half, half, **cache_args(k_scale=t)), torch.ones(5, 2)),
+        (lambda t: serving.cache_attention(t, **cache_args()), torch.zeros(3, 4, 64, dtype=BF16)),
+        (lambda t: serving.cache_attention(torch.zeros(3, 4, 64, dtype=BF16), **cache_args(v_scale=t)), torch.ones(5, 2)),
+        (lambda t: serving.token_logprobs(t, torch.zeros(2, dtype=torch.long)), torch.zeros(2, 9)),
+    ]
+    from torch.autograd import forward_ad
+
+    for call, t in calls:
+        with forward_ad.dual_level():
+            with pytest.raises(ValueError, match="tangent"):
+                call(forward_ad.make_dual(t, torch.ones_like(t)))
+            with pytest.raises(ValueError, match="on a GPU"):
+                call(t)
+        with pytest.raises(ValueError, match="tangent"):
+            torch.func.jvp(call, (t,), (torch.ones_like(t),))
+        with pytest.raises(ValueError, match="on a GPU"):
+            call(t)
+
+
 # -- the diagnostic that runs them -------------------------------------------
 
 

@@ -58,6 +58,7 @@ _MOST_PRODUCTS = 2**33
 _MOST_HEADS = 2**22  # heads of all sequences
 _MOST_HEAD_ROWS = 2**26  # (row, head) pairs
 _MOST_LOGIT_ROWS = 2**24 - 1
+_MOST_SCALE = torch.finfo(torch.float32).max
 
 GROUPS = (32, 64, 128)
 MAX_COLUMNS = _serving.MAX_COLUMNS
@@ -421,7 +422,7 @@ def cache_attention(
     rows are its last tokens, whose keys and values the cache holds already.
     A row at position p sees the positions up to p, with ``window`` only the
     last ``window`` of them. ``q_heads`` is a multiple of the cache's heads.
-    ``scale``, over 0, is dim ** -0.5 unless given. ``max_seq_len``, the longest length
+    ``scale``, over 0 and finite in float32, is dim ** -0.5 unless given. ``max_seq_len``, the longest length
     as far as the program knows it, only steers how work is split.
 
     Returns (out [T, q_heads, dim] in q's type, lse float32 [T, q_heads]), lse
@@ -447,8 +448,8 @@ def cache_attention(
         raise ValueError("more than 2^26 query rows")
     if scale is None:
         scale = dim**-0.5
-    elif not 0 < scale < math.inf:
-        raise ValueError(f"scale must be positive and finite, not {scale}")
+    elif not 0 < scale <= _MOST_SCALE:
+        raise ValueError(f"scale must be positive, and finite in float32, not {scale}")
     if window is not None and window < 1:
         raise ValueError(f"window must be at least 1, not {window}")
     room = cache[13] * cache[10]

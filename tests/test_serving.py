@@ -425,6 +425,18 @@ def test_tangents_are_refused():
             call(t)
 
 
+@pytest.mark.parametrize("scale", [1e39, 3.5e38, float("nan"), -0.1])
+def test_scales_past_float32_are_refused(scale):
+    with pytest.raises(ValueError, match="scale"):
+        serving.cache_attention(torch.zeros(3, 4, 64, dtype=BF16), **cache_args(), scale=scale)
+
+
+@pytest.mark.parametrize("scale", [3.4e38, 1e-46, 1, 0.125])
+def test_other_scales_are_taken(scale):
+    with pytest.raises(ValueError, match="on a GPU"):
+        serving.cache_attention(torch.zeros(3, 4, 64, dtype=BF16), **cache_args(), scale=scale)
+
+
 # -- the diagnostic that runs them -------------------------------------------
 
 

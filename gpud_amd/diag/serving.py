@@ -422,14 +422,18 @@ def cache_attention(
     rows are its last tokens, whose keys and values the cache holds already.
     A row at position p sees the positions up to p, with ``window`` only the
     last ``window`` of them. ``q_heads`` is a multiple of the cache's heads.
-    ``scale``, over 0 and finite in float32, is dim ** -0.5 unless given. ``max_seq_len``, the longest length
-    as far as the program knows it, only steers how work is split.
+    ``scale``, over 0 and finite in float32, is dim ** -0.5 unless given.
+    ``max_seq_len``, the longest length as far as the program knows it, only
+    steers how work is split.
 
     Returns (out [T, q_heads, dim] in q's type, lse float32 [T, q_heads]), lse
     the logarithm of the sum of the exponentials of a row's scores. The scales
     of pages that a row sees have to be positive and finite; others may hold
-    anything. A row that sees nothing gets 0 and -inf. A sequence whose pages are out of range, or
-    that is longer than its row of ``block_table``, gets NaN. Rows behind the
+    anything. The value scales of a sequence's head may differ by a factor of
+    2^100, which values under 2^44 (1e13) never pass, beside zeros either; queries
+    are under 2^110 (1e33) in magnitude. Beyond that fp32 does not hold a row's
+    sums. A row that sees nothing gets 0 and -inf. A sequence whose pages are out
+    of range, or that is longer than its row of ``block_table``, gets NaN. Rows behind the
     last sequence are left as they were in ``out`` if that is given, and else
     0; their lse is -inf. ``out`` may not share memory with the other arguments.
     """

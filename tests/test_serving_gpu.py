@@ -669,6 +669,26 @@ def test_attention_of_many_small_weights_beside_a_large_one(serving, rows):
         close(lse, torch.log(pos + sink), rel + 16 * 4 * E32)
 
 
+def test_attention_at_the_limits_of_its_values(serving):
+    lens, page = [70, 40], 16
+    cache = Cache(serving, lens, 2, 64, page)
+    g = gen(8)
+    k, v = (torch.randn(110, 2, 64, generator=g, device="cuda") for _ in range(2))
+    at = torch.cat([torch.arange(n, device="cuda") for n in lens])
+    v *= torch.where(at // page % 2 == 0, 0.0, 3e12)[:, None, None]
+    serving.cache_append(k.to(BF16), v.to(BF16), *cache.tensors, cache.table, ints(lens), ints(starts_of(lens)))
+    largest = cache.tensors[3].amax()
+    assert 2.0**-64 * 2.0**98 <= float(largest) <= 2.0**-64 * 2.0**100
+    q = torch.randn(2, 8, 64, generator=g, device="cuda").to(BF16)
+    check_attention(cache, q, lens, [0, 1, 2], serving.cache_attention(q, *cache.tensors, cache.table, ints(lens)))
+    q = torch.full_like(q, 2.0**109)  # scores of one sign and the largest size
+    key = torch.full((110, 2, 64), 1.75 * 2.0**-64 * 2.0**8, dtype=BF16, device="cuda")
+    serving.cache_append(key, v.to(BF16), *cache.tensors, cache.table, ints(lens), ints(starts_of(lens)))
+    assert bool((cache.tensors[2][cache.table[0].long()] == 2.0**-64).all())
+    got = serving.cache_attention(q, *cache.tensors, cache.table, ints(lens), scale=2.0**-60)
+    check_attention(cache, q, lens, [0, 1, 2], got, scale=2.0**-60)
+
+
 # ---------------------------------------------------------------------------
 # token_logprobs
 # ---------------------------------------------------------------------------

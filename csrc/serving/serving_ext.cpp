@@ -272,7 +272,7 @@ PyMethodDef launches[] = {
 // workgroup of attention has, and (slot, page, from, to, src) of every append.
 std::vector<std::vector<int64_t>> attention_places(const std::vector<int32_t>& starts, const std::vector<int32_t>& lens,
                                                    int rows, int heads, int q_heads, int page, int blocks, int window,
-                                                   int64_t max_seq_len, bool fill_tail) {
+                                                   int64_t max_seq_len, bool fill_tail, int dim) {
   AttentionArgs all{};
   all.c.starts = starts.empty() ? nullptr : starts.data();
   all.c.lens = lens.data();
@@ -281,7 +281,7 @@ std::vector<std::vector<int64_t>> attention_places(const std::vector<int32_t>& s
   all.c.heads = heads;
   all.c.page = page;
   all.c.blocks = blocks;
-  all.c.dim = 128;
+  all.c.dim = dim;
   all.q_heads = q_heads;
   all.window = window;
   all.tail = fill_tail ? kFillTail : kLeaveTail;
@@ -355,7 +355,9 @@ PYBIND11_MODULE(_serving, m) {
   m.def("serving_step", &step, py::arg("device") = 0, py::arg("iters") = 20, py::arg("seed") = 1,
         py::arg("oracle_offset") = 0.0,
         "One token step of a synthetic served model, checked against host oracles; returns rates + verification");
-  m.def("attention_places", &attention_places);
+  m.def("attention_places", &attention_places, py::arg("starts"), py::arg("lens"), py::arg("rows"), py::arg("heads"),
+        py::arg("q_heads"), py::arg("page"), py::arg("blocks"), py::arg("window"), py::arg("max_seq_len"),
+        py::arg("fill_tail"), py::arg("dim") = 128);
   m.def("append_places", &append_places);
   m.attr("MAX_COLUMNS") = kMaxColumns;
   m.attr("MAX_TOKENS") = kMaxTokens;

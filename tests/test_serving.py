@@ -111,6 +111,39 @@ def test_attention_gives_each_row_its_tokens_once(seed):
                 assert parts[-1][2] <= max(length, 0)
 
 
+@pytest.mark.parametrize("seed", range(40))
+def test_attention_of_any_dimension_gives_each_row_its_tokens_once(seed):
+    """Wide heads have tiles of 16 rows and more of them a sequence; single tokens too."""
+    rng = random.Random(seed)
+    dim, heads = rng.choice([16, 64, 80, 128, 144, 208, 256]), rng.choice([1, 3])
+    group = rng.choice([1, 3, 8, 16, 17, 32, 40, 64, 65, 130])
+    starts, lens = _random_batch(rng)
+    single = rng.random() < 0.3
+    if single:
+        starts = list(range(len(lens) + 1))
+    tail = 0 if single else rng.choice([0, 7])
+    rows = starts[-1] + tail
+    if not rows:
+        return
+    window = rng.choice([0, 1, 64, 100])
+    got = _serving.attention_places(
+        [] if single else starts, lens, rows, heads, heads * group, 16, 80, window, rng.choice([1, 700, 5000]), True, dim
+    )
+    spans = {}
+    for row, head, slot, split, lo, hi in got:
+        spans.setdefault((row, head), []).append((split, lo, hi))
+    assert set(spans) == {(r, h) for r in range(rows) for h in range(group)}
+    for b, length in enumerate(lens):
+        for i in range(starts[b], starts[b + 1]):
+            pos = length - starts[b + 1] + i
+            for h in range(group):
+                parts = sorted(spans[i, h])
+                assert [p[0] for p in parts] == list(range(len(parts)))
+                assert all(p[2] == q[1] for p, q in zip(parts, parts[1:]))
+                assert pos < 0 or parts[0][1] <= max(0, pos - window + 1 if window else 0) and parts[-1][2] > pos
+                assert parts[-1][2] <= max(length, 0)
+
+
 @pytest.mark.parametrize("seed", range(30))
 def test_attention_survives_any_starts_and_lengths(seed):
     """Broken metadata may leave rows out; it never names a row that is not there."""

@@ -332,6 +332,19 @@ def test_cache_append_leaves_out_bad_pages_and_other_rows(serving):
     serving.cache_append(k, k, *cache.tensors, table, ints([48 + 40, 0, -5]), ints([0, 40, 80, 120]))
 
 
+def test_cache_append_of_sequences_longer_than_their_table(serving):
+    """Their tokens up to its end are written, and nothing of empty ones or of negative lengths."""
+    heads, dim, page = 2, 32, 16
+    cache = Cache(serving, [40, 40, 40], heads, dim, page, spare=1)
+    mirror = [t.clone() for t in cache.tensors]
+    k = torch.randn(125, heads, dim, generator=gen(4), device="cuda").to(BF16)
+    lens, starts = [48 + 17, 0, -5], [0, 40, 80, 120]
+    serving.cache_append(k, -k, *cache.tensors, cache.table, ints(lens), ints(starts))
+    for i, x in ((0, k), (1, -k)):
+        plain_append(mirror[i], mirror[i + 2], x, cache.table.cpu()[:1], [48], [0, 48 - (65 - 40)], page, bool(i))
+        assert torch.equal(cache.tensors[i + 2], mirror[i + 2]) and same_codes(cache.tensors[i], mirror[i])
+
+
 # ---------------------------------------------------------------------------
 # cache_attention
 # ---------------------------------------------------------------------------

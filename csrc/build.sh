@@ -34,11 +34,15 @@ if [ -d csrc/serving ]; then
   mkdir -p build/serving
   pids=()
   for src in csrc/serving/*.hip csrc/serving/*.cpp; do
-    ${ROCM}/bin/hipcc ${HIPFLAGS} -O3 ${PYINC} -c "${src}" \
-        -o "build/serving/$(basename "${src}").o" &
+    out="build/serving/$(basename "${src}")"
+    ${ROCM}/bin/hipcc ${HIPFLAGS} -O3 ${PYINC} -Rpass-analysis=kernel-resource-usage \
+        -c "${src}" -o "${out}.o" 2> "${out}.log" &
     pids+=($!)
   done
-  for pid in "${pids[@]}"; do wait "${pid}"; done
+  for pid in "${pids[@]}"; do
+    wait "${pid}" || { grep -h -A5 "error:" build/serving/*.log >&2; exit 1; }
+  done
+  awk -f csrc/scalar_spills.awk build/serving/*.log >&2
   ${ROCM}/bin/hipcc --offload-arch=gfx950 -shared build/serving/*.o \
       -o gpud_amd/diag/_serving${PYEXT}
 fi

@@ -470,6 +470,29 @@ def test_other_scales_are_taken(scale):
         serving.cache_attention(torch.zeros(3, 4, 64, dtype=BF16), **cache_args(), scale=scale)
 
 
+# -- the build ---------------------------------------------------------------
+
+
+@pytest.mark.parametrize(
+    "spilled,said",
+    [((0, 0), ""), ((0, 3), "second spills 3 scalar"), ((54, 0), "first spills 54 scalar"), ((), "no resource remarks")],
+)
+def test_build_refuses_kernels_that_spill_scalar_registers(tmp_path, spilled, said):
+    import os
+    import subprocess
+
+    text = "attention.hip:9:1: warning: something else\n"
+    for name, n in zip(("first", "second"), spilled):
+        for line in (f"Function Name: {name}", "    SGPRs: 100", f"    SGPRs Spill: {n}", "    VGPRs Spill: 28"):
+            text += f"attention.hip:1:1: remark: {line} [-Rpass-analysis=kernel-resource-usage]\n"
+    log = tmp_path / "log"
+    log.write_text(text)
+    script = os.path.join(os.path.dirname(__file__), "..", "csrc", "scalar_spills.awk")
+    r = subprocess.run(["awk", "-f", script, str(log)], capture_output=True, text=True)
+    assert (r.returncode != 0) == bool(said) and said in r.stdout
+    assert said or not r.stdout
+
+
 # -- the diagnostic that runs them -------------------------------------------
 
 

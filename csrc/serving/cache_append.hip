@@ -16,7 +16,8 @@
 // us, 3.8 TB/s read and written of the 4.9 that a large copy reaches. Of single
 // tokens, one wave owns a sequence's head, half of it the key and half the
 // value; 256 of them take 7 us, bound by the chain of loads from the length to
-// the page's scale.
+// the page's scale. Where a scale grows, the half wave re-rounds its page a dword a
+// lane and turn: 15 us more for a page of 64 tokens by 128, 90 for 128 by 256.
 #include "device.h"
 #include "geometry.h"
 #include "serving.h"

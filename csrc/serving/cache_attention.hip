@@ -29,9 +29,10 @@
 // Measured, kernel and join: 64 contexts of 8000 to 16384 tokens, 64 heads on 8 of
 // 128: 275 + 6 us, 5.7 TB/s of the 6.3 that a plain read reaches (all heads of a
 // page on one die took it from 323 to 302, fewer workgroups to 280: split()); 32
-// of up to 4100 tokens: 32 + 3 us, bound by the latency of a workgroup's few tiles. A prompt of 4096 causal tokens, 32 heads on 8: 245 us,
-// 0.57 PFLOP/s; 4 chunks of 512 tokens on 8192: 350 us, 0.76 PFLOP/s, bound by the
-// vector unit's share of the softmax beside the matrix instructions.
+// of up to 4100 tokens: 32 + 3 us, bound by the latency of a workgroup's few tiles. A
+// prompt of 4096 causal tokens, 32 heads on 8: 215 us, 0.64 PFLOP/s; 4 chunks of 512
+// tokens on 8192: 304 us, 0.88 PFLOP/s, bound by the vector unit's share of the
+// softmax beside the matrix instructions.
 #include <type_traits>
 
 #include "device.h"

@@ -12,10 +12,10 @@ step against a host oracle; here they take a program's own tensors.
 * :func:`token_logprobs` - log probabilities of given tokens, with entropy,
   rank and the top alternatives
 
-All work is enqueued on the current stream of the tensors' device; nothing
-waits for the GPU, and results do not depend on timing. Every call may be
+All work is enqueued on the current stream of the tensors' device; these four
+never wait for the GPU, and results do not depend on timing. Each may be
 captured into a graph: workspaces are allocated per call from torch's
-allocator, so two graphs share none. Arguments that do not fit raise
+allocator, so two graphs share none. (:func:`pack_w4` waits for its checks.) Arguments that do not fit raise
 ``TypeError`` or ``ValueError`` before anything is enqueued. Page numbers,
 lengths and tokens that live on the GPU are bounded there: see each function.
 Tensors that have a shape but no memory (freed storages, fake tensors, wrapper
